@@ -1,9 +1,9 @@
 """mor_b200 -- B200 (sm_100a) implementation of the MoR fake-quantization operators.
 
-``import mor_b200`` loads ``libmor_b200.so`` (CUDA kernels behind a C ABI) and the
+``import mor_b200`` loads ``libmor_b200.so`` and ``libmor_b200_mx.so`` (CUDA kernels behind C ABIs) and the
 ``_C`` PyTorch shim, which registers ``torch.ops.mor.*`` with the operator schemas of
 boryiings/mor, and exposes ``mor_b200.ops`` with the signatures of ``mor/ops.py``.
-Both native artefacts must have been built (``python mor_b200/build.py``); importing
+All native artefacts must have been built (``python mor_b200/build.py``); importing
 fails loudly otherwise, and the operators exist for CUDA tensors only.
 """
 import torch  # noqa: F401  (the shim links against libtorch)
@@ -11,6 +11,7 @@ import torch  # noqa: F401  (the shim links against libtorch)
 from . import cabi
 
 cabi.lib()  # fail here, not at first use, if the kernels are not built
+cabi.mx_lib()
 
 try:
     from . import _C  # noqa: F401  registers torch.ops.mor.*

@@ -1,7 +1,8 @@
-"""ctypes binding of ``libmor_b200.so`` (the C ABI declared in ``include/mor_b200.h``).
+"""ctypes binding of ``libmor_b200.so`` (the C ABI declared in ``include/mor_b200.h``) and of
+``libmor_b200_mx.so`` (``include/mor_b200_mx.h``).
 
-This is what a host runtime without PyTorch would bind.  The library is loaded from
-this directory; if it is missing the import fails -- there is no CPU fallback.
+This is what a host runtime without PyTorch would bind.  The libraries are loaded from
+this directory; if one is missing the import fails -- there is no CPU fallback.
 Pointers are plain integers (``tensor.data_ptr()``), the stream is a ``cudaStream_t``
 handle as an integer (``torch.cuda.current_stream().cuda_stream``).
 """
@@ -12,9 +13,11 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmor_b200.so")
+MX_LIB_PATH = os.path.join(_HERE, "libmor_b200_mx.so")
 
 BF16, FP32 = 0, 1
 E4M3, E5M2, E3M2, E2M3 = 0, 1, 2, 3
+E2M1 = 4
 SF_FP32, SF_E8 = 1, 2
 OP_BLOCK_SCALING, OP_CHANNEL_SCALING, OP_E8MX, OP_AMAX_NNZ = 1, 2, 3, 4
 
@@ -57,6 +60,13 @@ SIGNATURES = {
     "mor_b200_p2p_exchange_errors": (_i, [_vp, _i64, _vp, _vp, _i, _i, C.c_uint32, _vp, _vp]),
 }
 
+# the entry points of include/mor_b200_mx.h
+MX_SIGNATURES = {
+    "mor_b200_mx_quantize_fp4": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "mor_b200_mx_dequantize": (_i, [_vp, _vp, _vp, _i, _i64, _i64, _i, _i, _vp]),
+    "mor_b200_mx_matmul": (_i, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i, _i, _vp, _vp, _vp]),
+    "mor_b200_mx_matmul_grad": (_i, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i, _i, _vp, _vp]),
+}
 
 ERR_UNSUPPORTED_SHAPE = -2   # MOR_B200_ERR_UNSUPPORTED_SHAPE
 
@@ -70,6 +80,7 @@ class MorB200Error(RuntimeError):
 
 
 _lib = None
+_mx_lib = None
 
 
 def lib() -> C.CDLL:
@@ -89,9 +100,26 @@ def lib() -> C.CDLL:
     return _lib
 
 
+def mx_lib() -> C.CDLL:
+    """Load libmor_b200_mx.so.  Raises if it has not been built: no fallback exists."""
+    global _mx_lib
+    if _mx_lib is None:
+        if not os.path.exists(MX_LIB_PATH):
+            raise ImportError(
+                f"{MX_LIB_PATH} is missing: build it with `python mor_b200/build.py` "
+                "(nvcc, sm_100a).  mor_b200 has no CPU or PyTorch fallback.")
+        L = C.CDLL(MX_LIB_PATH)
+        for name, (res, args) in MX_SIGNATURES.items():
+            fn = getattr(L, name)
+            fn.restype = res
+            fn.argtypes = args
+        _mx_lib = L
+    return _mx_lib
+
+
 def call(name: str, *args) -> None:
     """Invoke an int-status entry point and raise MorB200Error on failure."""
-    rc = getattr(lib(), name)(*args)
+    rc = getattr(mx_lib() if name in MX_SIGNATURES else lib(), name)(*args)
     if rc != 0:
         raise MorB200Error(name, rc, lib().mor_b200_status_string(rc).decode())
 

@@ -1,0 +1,312 @@
+// Product of two microscaled matrices, out[m, n] = sum_k A[m, k] B[n, k] + bias[n], on the block-scaled tensor core.
+//
+// Both operands are K-major with one E8M0 byte for every 32 elements of a row, which is what the instruction multiplies
+// into the product itself: the codes go from global to shared memory by TMA and are never widened.  A tile is 128 rows of
+// one operand (P) by TN rows of the other (Q), 128 bytes of K (256 E2M1 or 128 E4M3 / E5M2 elements) at a time.
+#include "mx_kernels.cuh"
+#include "tcgen05.cuh"
+
+namespace morb {
+namespace {
+
+struct MmArgs {
+    const uint8_t *sp, *sq;   // scale bytes of P and Q
+    const uint16_t* bias;
+    uint16_t* out;
+    int64_t p_rows, q_rows;
+    int64_t groups;           // scale bytes a row (K / 32)
+    int64_t ldo;              // row pitch of out (= n)
+    int64_t p_tiles;
+    uint32_t idesc;
+    int ktiles, splits, fast_scales, vec_out;
+};
+
+constexpr int kPRows = 128;
+
+template <bool FP4, int TN>
+struct MmShape {
+    static constexpr int kBlk = FP4 ? 2 : 1;                       // 512-byte scale blocks (128 rows x 4 groups) of P per step
+    static constexpr int kQBlk = kBlk * ((TN + 127) / 128);
+    static constexpr int kPBytes = kPRows * 128, kQBytes = TN * 128;
+    static constexpr int kSfOff = kPBytes + kQBytes;
+    static constexpr int kStage = (kSfOff + (kBlk + kQBlk) * 512 + 1023) & ~1023;
+    static constexpr int kStages = (200 * 1024) / kStage < 8 ? (200 * 1024) / kStage : 8;
+    static constexpr int kSmem = kStages * kStage + 1024;          // more than half of an SM: one CTA each, so the columns of tensor memory suffice
+    static constexpr int kSfCols = 4 * (kBlk + kQBlk);
+    static constexpr int kNeed = TN + 2 * kSfCols;
+    static constexpr int kCols = kNeed <= 64 ? 64 : (kNeed <= 128 ? 128 : (kNeed <= 256 ? 256 : 512));
+    static_assert(kSmem > 114 * 1024, "one CTA per SM");
+};
+
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Scale bytes of one row for one step: four a block, to the place the tensor core's copy takes them from (row r of 128:
+// 16 bytes for each r mod 32, four for each r / 32).  Rows and groups outside read as zero, a finite scale.
+template <int BLK>
+__device__ __forceinline__ void load_scales(uint32_t dst, const uint8_t* s, int64_t row, int64_t rows, int64_t groups, int64_t g0, bool fast) {
+#pragma unroll
+    for (int b = 0; b < BLK; ++b) {
+        const int64_t g = g0 + 4 * b;
+        const bool in = row < rows && g < groups;
+        const uint8_t* src = s + (in ? row * groups + g : 0);
+        if (fast) {
+            cp_async4(dst + b * 512, src, in ? 4 : 0);
+        } else {
+            uint32_t w = 0;
+            if (in) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (g + i < groups) w |= (uint32_t)__ldg(src + i) << (8 * i);
+            }
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + b * 512), "r"(w) : "memory");
+        }
+    }
+}
+
+// SWAP: P is B (rows of out's columns) and Q is A, so that few tokens fill a narrow tile of many weight rows.
+template <bool FP4, int TN, bool SWAP>
+__global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                                                           const MmArgs a) {
+    using S = MmShape<FP4, TN>;
+    constexpr int kLag = S::kStages - 1 < 4 ? S::kStages - 1 : 4;
+    constexpr int kGroupsPerStep = FP4 ? 8 : 4;
+    extern __shared__ uint8_t s_raw[];
+    __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], acc_done, drained;
+    __shared__ uint32_t s_tmem;
+    uint8_t* smem = s_raw + ((1024 - (smem_u32(s_raw) & 1023)) & 1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    const int split = (int)(blockIdx.x % (unsigned)a.splits);
+    const int64_t tile = blockIdx.x / (unsigned)a.splits;
+    const int64_t p0 = (tile % a.p_tiles) * kPRows, q0 = (tile / a.p_tiles) * TN;
+    const int k_first = (int)((int64_t)a.ktiles * split / a.splits), k_last = (int)((int64_t)a.ktiles * (split + 1) / a.splits);
+    const int n = k_last - k_first;
+
+    if (warp == 4 && lane == 0) {
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(&full[s], 1 + 4); mbar_init(&empty[s], 1); }
+        mbar_init(&acc_done, 1);
+        mbar_init(&drained, 1);
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_p));
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q));
+    }
+    if (warp == 5) tmem_alloc<1>(&s_tmem, S::kCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    bool ok = true;   // a wait that ran out ends the role's loop; the tile is then written as NaN
+    if (warp == 4) {
+        if (lane == 0) {
+            int i = 0;
+            for (; i < n && ok; ++i) {
+                const int s = i % S::kStages;
+                if (i >= S::kStages) ok = mbar_wait_bounded(&empty[s], (i / S::kStages - 1) & 1);
+                if (!ok) break;
+                uint8_t* st = smem + s * S::kStage;
+                mbar_expect_tx(&full[s], S::kPBytes + S::kQBytes);
+                const int x = (k_first + i) * 128;
+                tma_load_2d(st, &map_p, x, (int)p0, &full[s]);
+                tma_load_2d(st + S::kPBytes, &map_q, x, (int)q0, &full[s]);
+            }
+            if (!ok)   // copies in flight land before the shared memory is handed on
+                for (int j = i > S::kStages ? i - S::kStages : 0; j < i; ++j) mbar_wait_bounded(&full[j % S::kStages], (j / S::kStages) & 1);
+        }
+        __syncwarp();
+    } else if (warp == 5) {
+        if (lane == 0) {
+            for (int i = 0; i < n; ++i) {
+                const int s = i % S::kStages;
+                ok = mbar_wait_bounded(&full[s], (i / S::kStages) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t st = smem_u32(smem + s * S::kStage);
+                const uint32_t sfp = tmem + TN + (i & 1) * S::kSfCols, sfq = sfp + 4 * S::kBlk;
+#pragma unroll
+                for (int b = 0; b < S::kBlk + S::kQBlk; ++b) tc_copy_scales<1>(sfp + 4 * b, st + S::kSfOff + 512 * b);
+                const uint64_t dp = umma_desc_kmajor(st), dq = umma_desc_kmajor(st + S::kPBytes);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {   // 32 bytes of K each
+                    const uint32_t blk = FP4 ? k >> 1 : 0, id = FP4 ? (k & 1) * 2 : k;
+                    tc_mma_scaled<1, FP4>(tmem, dp + 2 * k, dq + 2 * k, idesc_with_scale_id(a.idesc, id), sfp + 4 * blk,
+                                          sfq + 4 * blk * ((TN + 127) / 128), (i | k) != 0);
+                }
+                tc_commit(&empty[s]);
+            }
+            tc_commit(ok ? &acc_done : &drained);
+            if (!ok) mbar_wait_bounded(&drained, 0);
+        }
+        __syncwarp();
+    } else {
+        const int t = threadIdx.x;   // 0..127
+        const uint32_t place = (t & 31) * 16 + (t >> 5) * 4;
+        for (int i = 0; i < n + kLag; ++i) {
+            if (i < n) {
+                const int s = i % S::kStages;
+                if (i >= S::kStages) ok = mbar_wait_bounded(&empty[s], (i / S::kStages - 1) & 1);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) break;
+                const uint32_t sf = smem_u32(smem + s * S::kStage + S::kSfOff) + place;
+                const int64_t g0 = (int64_t)(k_first + i) * kGroupsPerStep;
+                load_scales<S::kBlk>(sf, a.sp, p0 + t, a.p_rows, a.groups, g0, a.fast_scales);
+#pragma unroll
+                for (int h = 0; h < (TN + 127) / 128; ++h)
+                    if (h * 128 + t < TN)
+                        load_scales<S::kBlk>(sf + 512 * (S::kBlk + h), a.sq, q0 + h * 128 + t, a.q_rows, a.groups, g0, a.fast_scales);
+            }
+            cp_async_commit();
+            if (i >= kLag) {
+                cp_async_wait<kLag>();
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[(i - kLag) % S::kStages]);
+            }
+        }
+        cp_async_wait<0>();
+        ok = ok && mbar_wait_bounded(&acc_done, 0);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        tc_fence_after();
+    }
+
+    if (warp < 4) {
+        const uint32_t lanes = tmem + ((uint32_t)warp << 21);   // lane field of the address: 32 per warp
+        const float bad = u2f(0x7FFFFFFFu);
+        constexpr int C = TN < 32 ? 16 : 32;
+        const int64_t p = p0 + threadIdx.x;
+#pragma unroll 1
+        for (int c0 = 0; c0 < TN; c0 += C) {
+            uint32_t r[C];
+            if constexpr (C == 32) tmem_load32(lanes + c0, r); else tmem_load16(lanes + c0, r);
+            tmem_wait_loads();
+            if (!ok) {
+#pragma unroll
+                for (int c = 0; c < C; ++c) r[c] = f2u(bad);
+            }
+            if (a.splits > 1) {
+                float* part = reinterpret_cast<float*>(smem);   // [column][128 rows]; the operands are no longer needed
+#pragma unroll
+                for (int c = 0; c < C; ++c) part[(c0 + c) * kPRows + threadIdx.x] = u2f(r[c]);
+            } else if (p < a.p_rows) {
+                if constexpr (SWAP) {
+                    const float b = a.bias ? u2f((uint32_t)__ldg(a.bias + p) << 16) : 0.0f;
+#pragma unroll
+                    for (int c = 0; c < C; ++c)
+                        if (q0 + c0 + c < a.q_rows) a.out[(q0 + c0 + c) * a.ldo + p] = (uint16_t)pack_bf16_rne(0.0f, u2f(r[c]) + b);
+                } else {
+                    const int64_t q = q0 + c0;
+                    uint16_t* o = a.out + p * a.ldo + q;
+                    if (a.bias) {
+#pragma unroll
+                        for (int c = 0; c < C; ++c)
+                            if (q + c < a.q_rows) r[c] = f2u(u2f(r[c]) + u2f((uint32_t)__ldg(a.bias + q + c) << 16));
+                    }
+                    if (a.vec_out && q + C <= a.q_rows) {
+#pragma unroll
+                        for (int c = 0; c < C; c += 8)
+                            *reinterpret_cast<uint4*>(o + c) = make_uint4(
+                                pack_bf16_rne(u2f(r[c + 1]), u2f(r[c])), pack_bf16_rne(u2f(r[c + 3]), u2f(r[c + 2])),
+                                pack_bf16_rne(u2f(r[c + 5]), u2f(r[c + 4])), pack_bf16_rne(u2f(r[c + 7]), u2f(r[c + 6])));
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < C; ++c)
+                            if (q + c < a.q_rows) o[c] = (uint16_t)pack_bf16_rne(0.0f, u2f(r[c]));
+                    }
+                }
+            }
+        }
+    }
+    if (a.splits > 1) {   // the CTAs of a cluster hold partial sums of one tile: each adds up some of the columns, in rank order
+        cluster_sync();
+        if (warp < 4) {
+            const int64_t p = p0 + threadIdx.x;
+            const uint32_t mine = smem_u32(smem) + 4 * threadIdx.x;
+            for (int c = split; c < TN && q0 + c < a.q_rows; c += a.splits) {
+                float sum = 0.0f;
+                for (int z = 0; z < a.splits; ++z) {
+                    float v;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(mine + c * (kPRows * 4), z)) : "memory");
+                    sum += v;
+                }
+                if (p < a.p_rows) {
+                    const int64_t col = SWAP ? p : q0 + c, row = SWAP ? q0 + c : p;
+                    if (a.bias) sum += u2f((uint32_t)__ldg(a.bias + col) << 16);
+                    a.out[row * a.ldo + col] = (uint16_t)pack_bf16_rne(0.0f, sum);
+                }
+            }
+        }
+        cluster_sync();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 5) { tc_fence_after(); tmem_free<1>(tmem, S::kCols); }
+}
+
+template <bool FP4, int TN, bool SWAP>
+int go(const CUtensorMap& mp, const CUtensorMap& mq, const MmArgs& a, int64_t tiles, cudaStream_t st) {
+    using S = MmShape<FP4, TN>;
+    auto k = mx_matmul_kernel<FP4, TN, SWAP>;
+    static SmemOptIn opt;
+    if (!opt(k, S::kSmem)) return kErrLaunch;
+    if (tiles * a.splits > 0x7FFFFFFF) return kErrTooLarge;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * a.splits));
+    cfg.blockDim = dim3(192);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {(unsigned)a.splits, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = a.splits > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, k, mp, mq, a) == cudaSuccess ? check_launch() : kErrLaunch;
+}
+
+template <bool FP4>
+int dispatch(const MxMatmulArgs& x, cudaStream_t st) {
+    const bool swap = x.m <= 64;
+    const int tn = !swap ? 128 : (x.m <= 16 ? 16 : (x.m <= 32 ? 32 : 64));
+    MmArgs a = {};
+    const void *p = swap ? x.b : x.a, *q = swap ? x.a : x.b;
+    a.sp = swap ? x.b_scales : x.a_scales;
+    a.sq = swap ? x.a_scales : x.b_scales;
+    a.p_rows = swap ? x.n : x.m;
+    a.q_rows = swap ? x.m : x.n;
+    a.bias = static_cast<const uint16_t*>(x.bias);
+    a.out = static_cast<uint16_t*>(x.out);
+    a.groups = x.k / 32;
+    a.ldo = x.n;
+    a.p_tiles = (a.p_rows + kPRows - 1) / kPRows;
+    const int64_t row_bytes = FP4 ? x.k / 2 : x.k;
+    a.ktiles = (int)((row_bytes + 127) / 128);
+    const int pf = swap ? x.b_fmt : x.a_fmt, qf = swap ? x.a_fmt : x.b_fmt;
+    a.idesc = idesc_scaled(128, tn, FP4 ? 1u : (uint32_t)pf, FP4 ? 1u : (uint32_t)qf);
+    a.fast_scales = a.groups % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.sp) | reinterpret_cast<uintptr_t>(a.sq)) & 3) == 0;
+    a.vec_out = x.n % 8 == 0 && (reinterpret_cast<uintptr_t>(x.out) & 15) == 0;
+    const int64_t tiles = a.p_tiles * ((a.q_rows + tn - 1) / tn);
+    a.splits = 1;
+    while (a.splits < 8 && tiles * a.splits * 2 <= sm_count() && a.ktiles >= a.splits * 4) a.splits *= 2;
+    CUtensorMap mp, mq;
+    if (!make_swizzled_map(&mp, p, a.p_rows, row_bytes, row_bytes, 1, kPRows)) return kErrLaunch;
+    if (!make_swizzled_map(&mq, q, a.q_rows, row_bytes, row_bytes, 1, tn)) return kErrLaunch;
+    if (!swap) return go<FP4, 128, false>(mp, mq, a, tiles, st);
+    if (tn == 16) return go<FP4, 16, true>(mp, mq, a, tiles, st);
+    if (tn == 32) return go<FP4, 32, true>(mp, mq, a, tiles, st);
+    return go<FP4, 64, true>(mp, mq, a, tiles, st);
+}
+
+}  // namespace
+
+int launch_mx_matmul(const MxMatmulArgs& x, cudaStream_t st) {
+    return x.a_fmt == kE2M1 ? dispatch<true>(x, st) : dispatch<false>(x, st);
+}
+
+}  // namespace morb

@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "../../include/mor_b200.h"
+#include "../../include/mor_b200_mx.h"
 
 namespace mor {
 
@@ -333,6 +334,113 @@ std::vector<at::Tensor> quantize_scaled(const at::Tensor& input, int64_t rows, i
     return {payload, scales, gamax};
 }
 
+// ---- extension: microscaled operands (include/mor_b200_mx.h) -----------------------------
+// One code per element, or two to a byte for E2M1; the tensors of one operand lie on one device.
+bool mx_format_ok(int64_t f) { return f == MOR_B200_E4M3 || f == MOR_B200_E5M2 || f == MOR_B200_E2M3 || f == MOR_B200_MX_E2M1; }
+
+at::Tensor mx_part(const at::Tensor& t, int64_t rows, int64_t cols, const at::Tensor& like, size_t align, const char* op, const char* what) {
+    TORCH_CHECK(t.is_cuda() && t.device() == like.device(), "mor::", op, ": ", what, " must be on ", like.device());
+    TORCH_CHECK(t.scalar_type() == at::kByte, "mor::", op, ": ", what, " must be uint8");
+    TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols, "mor::", op, ": ", what, " must be [", rows, ", ", cols, "]");
+    at::Tensor c = t.contiguous();
+    if (reinterpret_cast<uintptr_t>(c.data_ptr()) % align) c = c.clone();
+    return c;
+}
+at::Tensor mx_payload(const at::Tensor& t, int64_t rows, int64_t cols, int64_t format, const at::Tensor& like, const char* op, const char* what) {
+    return mx_part(t, rows, format == MOR_B200_MX_E2M1 ? cols / 2 : cols, like, 16, op, what);
+}
+// rows as they are where the copy engine can take them (unit stride along a row, rows a multiple of 16 bytes apart), packed otherwise
+at::Tensor mx_rows(const at::Tensor& t, int64_t& pitch) {
+    const int64_t w = t.element_size(), packed = (t.size(1) * w + 15) / 16 * 16 / w;
+    pitch = t.size(0) > 1 ? t.stride(0) : packed;
+    const bool unit = t.stride(1) == 1 || t.size(1) == 1;
+    if (unit && pitch >= t.size(1) && pitch * w % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) return t;
+    pitch = packed;
+    at::Tensor p = torch::empty({t.size(0), packed}, t.options());
+    p.narrow(1, 0, t.size(1)).copy_(t);
+    return p;
+}
+
+// returns [payload uint8 [dim_x, dim_y / 2], scales uint8 [dim_x, dim_y / 32]]
+std::vector<at::Tensor> quantize_mx_fp4(const at::Tensor& input, int64_t rows, int64_t cols, int64_t bc) {
+    TORCH_CHECK(input.is_cuda(), "mor::quantize_mx_fp4: input must be a CUDA tensor");
+    const c10::cuda::CUDAGuard guard(input.device());
+    TORCH_CHECK(input.dim() == 2 && input.size(0) == rows && input.size(1) == cols,
+                "mor::quantize_mx_fp4: input must be [dim_x, dim_y] = [", rows, ", ", cols, "]");
+    const int dt = dtype_code(input, true, "quantize_mx_fp4");
+    TORCH_CHECK(bc == 32, "mor::quantize_mx_fp4: block_y must be 32");
+    TORCH_CHECK(cols > 0 && cols % 32 == 0, "mor::quantize_mx_fp4: dim_y must be a positive multiple of 32");
+    at::Tensor payload = torch::empty({rows, cols / 2}, input.options().dtype(torch::kUInt8));
+    at::Tensor scales = torch::empty({rows, cols / 32}, input.options().dtype(torch::kUInt8));
+    if (rows == 0) return {payload, scales};
+    int64_t pitch = 0;
+    at::Tensor in = mx_rows(input, pitch);
+    check_status(mor_b200_mx_quantize_fp4(in.data_ptr(), dt, rows, cols, pitch, payload.data_ptr(), scales.data_ptr(), cur_stream()),
+                 "quantize_mx_fp4");
+    return {payload, scales};
+}
+
+at::Tensor dequantize_mx(const at::Tensor& payload, const at::Tensor& scales, int64_t rows, int64_t cols, int64_t bc, int64_t format,
+                         at::ScalarType dtype) {
+    TORCH_CHECK(payload.is_cuda(), "mor::dequantize_mx: payload must be a CUDA tensor");
+    const c10::cuda::CUDAGuard guard(payload.device());
+    TORCH_CHECK(mx_format_ok(format), "mor::dequantize_mx: elem_format must be 0 (E4M3), 1 (E5M2), 3 (E2M3) or 4 (E2M1)");
+    TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kFloat, "mor::dequantize_mx: out_dtype must be bfloat16 or float32");
+    TORCH_CHECK(rows >= 0 && cols > 0 && bc >= 8 && bc <= 256 && (bc & (bc - 1)) == 0 && cols % bc == 0,
+                "mor::dequantize_mx: block_y must be a power of two from 8 to 256 that divides dim_y");
+    at::Tensor p = mx_payload(payload, rows, cols, format, payload, "dequantize_mx", "payload");
+    at::Tensor s = mx_part(scales, rows, cols / bc, payload, 1, "dequantize_mx", "scales");
+    at::Tensor out = torch::empty({rows, cols}, payload.options().dtype(dtype));
+    check_status(mor_b200_mx_dequantize(p.data_ptr(), s.data_ptr(), out.data_ptr(), dtype == at::kFloat ? MOR_B200_FP32 : MOR_B200_BF16,
+                                        rows, cols, (int)bc, (int)format, cur_stream()),
+                 "dequantize_mx");
+    return out;
+}
+
+at::Tensor mx_matmul(const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& b, const at::Tensor& b_scales, int64_t m, int64_t n,
+                     int64_t k, int64_t a_format, int64_t b_format, const std::optional<at::Tensor>& bias) {
+    TORCH_CHECK(a.is_cuda(), "mor::mx_matmul: a must be a CUDA tensor");
+    const c10::cuda::CUDAGuard guard(a.device());
+    const bool fp4 = a_format == MOR_B200_MX_E2M1 && b_format == MOR_B200_MX_E2M1;
+    const bool fp8 = (a_format == MOR_B200_E4M3 || a_format == MOR_B200_E5M2) && (b_format == MOR_B200_E4M3 || b_format == MOR_B200_E5M2);
+    TORCH_CHECK(fp4 || fp8, "mor::mx_matmul: formats must be 4 and 4 (E2M1), or each 0 (E4M3) or 1 (E5M2)");
+    TORCH_CHECK(m >= 0 && n >= 0 && k > 0 && k % 32 == 0, "mor::mx_matmul: dim_k must be a positive multiple of 32");
+    at::Tensor ac = mx_payload(a, m, k, a_format, a, "mx_matmul", "a"), as = mx_part(a_scales, m, k / 32, a, 1, "mx_matmul", "a_scales");
+    at::Tensor bcod = mx_payload(b, n, k, b_format, a, "mx_matmul", "b"), bs = mx_part(b_scales, n, k / 32, a, 1, "mx_matmul", "b_scales");
+    at::Tensor bi;
+    if (bias.has_value() && bias->defined()) {
+        TORCH_CHECK(bias->is_cuda() && bias->device() == a.device() && bias->scalar_type() == at::kBFloat16 && bias->dim() == 1 && bias->size(0) == n,
+                    "mor::mx_matmul: bias must be bfloat16 [dim_n] on ", a.device());
+        bi = bias->contiguous();
+    }
+    at::Tensor out = torch::empty({m, n}, a.options().dtype(torch::kBFloat16));
+    check_status(mor_b200_mx_matmul(ac.data_ptr(), as.data_ptr(), bcod.data_ptr(), bs.data_ptr(), m, n, k, (int)a_format, (int)b_format,
+                                    bi.defined() ? bi.data_ptr() : nullptr, out.data_ptr(), cur_stream()),
+                 "mx_matmul");
+    return out;
+}
+
+at::Tensor mx_matmul_grad(const at::Tensor& g, const at::Tensor& payload, const at::Tensor& scales, int64_t m, int64_t n, int64_t k,
+                          int64_t format, bool transpose_g) {
+    TORCH_CHECK(g.is_cuda(), "mor::mx_matmul_grad: g must be a CUDA tensor");
+    const c10::cuda::CUDAGuard guard(g.device());
+    TORCH_CHECK(mx_format_ok(format), "mor::mx_matmul_grad: elem_format must be 0 (E4M3), 1 (E5M2), 3 (E2M3) or 4 (E2M1)");
+    TORCH_CHECK(m >= 0 && n >= 0 && k >= 0 && n % 32 == 0, "mor::mx_matmul_grad: dim_n must be a multiple of 32");
+    TORCH_CHECK(g.scalar_type() == at::kBFloat16, "mor::mx_matmul_grad: g must be bfloat16");
+    TORCH_CHECK(g.dim() == 2 && g.size(0) == (transpose_g ? k : m) && g.size(1) == (transpose_g ? m : k),
+                "mor::mx_matmul_grad: g must be [dim_m, dim_k], or [dim_k, dim_m] with transpose_g");
+    at::Tensor p = mx_payload(payload, k, n, format, g, "mx_matmul_grad", "payload");
+    at::Tensor s = mx_part(scales, k, n / 32, g, 1, "mx_matmul_grad", "scales");
+    at::Tensor out = torch::empty({m, n}, g.options());
+    if (m == 0 || n == 0) return out;
+    int64_t pitch = 0;
+    at::Tensor gr = mx_rows(g, pitch);
+    check_status(mor_b200_mx_matmul_grad(gr.data_ptr(), pitch, p.data_ptr(), s.data_ptr(), m, n, k, (int)format, transpose_g ? 1 : 0,
+                                         out.data_ptr(), cur_stream()),
+                 "mx_matmul_grad");
+    return out;
+}
+
 }  // namespace
 
 // Registers _C as a Python extension module.
@@ -361,6 +469,11 @@ TORCH_LIBRARY(mor, m) {
   m.def("quantize_scaled(Tensor input, int dim_x, int dim_y, int block_x, int block_y, int ss_mode) -> Tensor[]");
   m.def("fake_quantize_block_scaling_delayed(Tensor input, int dim_x, int dim_y, int block_x, int block_y, float e4m3_threshold, int ss_mode, Tensor amax_in) -> Tensor[]");
   m.def("fake_quantize_block_scaling_delayed_t(Tensor input, int dim_x, int dim_y, int block_x, int block_y, float e4m3_threshold, int ss_mode, Tensor amax_in) -> Tensor[]");
+  // microscaled operands: 4-bit codes, codes back to values, products
+  m.def("quantize_mx_fp4(Tensor input, int dim_x, int dim_y, int block_y) -> Tensor[]");
+  m.def("dequantize_mx(Tensor payload, Tensor scales, int dim_x, int dim_y, int block_y, int elem_format, ScalarType out_dtype) -> Tensor");
+  m.def("mx_matmul(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, int dim_m, int dim_n, int dim_k, int a_format, int b_format, Tensor? bias) -> Tensor");
+  m.def("mx_matmul_grad(Tensor g, Tensor payload, Tensor scales, int dim_m, int dim_n, int dim_k, int elem_format, bool transpose_g) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(mor, CUDA, m) {
@@ -384,6 +497,10 @@ TORCH_LIBRARY_IMPL(mor, CUDA, m) {
   m.impl("quantize_scaled", &quantize_scaled);
   m.impl("fake_quantize_block_scaling_delayed", &fake_quantize_block_scaling_delayed);
   m.impl("fake_quantize_block_scaling_delayed_t", &fake_quantize_block_scaling_delayed_t);
+  m.impl("quantize_mx_fp4", &quantize_mx_fp4);
+  m.impl("dequantize_mx", &dequantize_mx);
+  m.impl("mx_matmul", &mx_matmul);
+  m.impl("mx_matmul_grad", &mx_matmul_grad);
 }
 
 }  // namespace mor

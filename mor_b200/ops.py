@@ -9,7 +9,7 @@ argument gets ``None`` (mor/ops.py:15-21 and the registrations that follow it).
 """
 from __future__ import annotations
 
-from typing import List
+from typing import List, Optional
 
 import torch
 from torch import Tensor
@@ -29,6 +29,7 @@ __all__ = [
     "quantize_scaled",
     "fake_quantize_block_scaling_delayed",
     "fake_quantize_block_scaling_delayed_t",
+    "quantize_mx_fp4", "dequantize_mx", "mx_matmul", "mx_matmul_grad",
 ]
 
 
@@ -172,6 +173,41 @@ def quantize_scaled(a: Tensor, dim_x: int, dim_y: int, block_x: int, block_y: in
     (``uint8 [dim_x, dim_y]``, viewable as ``torch.float8_e4m3fn``), one ``float32`` scale per block
     (``[dim_x // block_x, dim_y // block_y]``) and the tensor's amax; ``element = decode(code) / scale``.  No gradient."""
     return _ops.quantize_scaled.default(a, dim_x, dim_y, block_x, block_y, ss_mode)
+
+
+# --------------------------------------------------------------------------- microscaled operands
+# An MX matrix is a payload of codes and one E8M0 byte per group of columns, as quantize_mx returns them; formats:
+# 0 E4M3, 1 E5M2, 3 E2M3 (a byte each), 4 E2M1 (two to a byte, the even column in the low half).
+def quantize_mx_fp4(a: Tensor, dim_x: int, dim_y: int, block_y: int) -> List[Tensor]:
+    """4-bit form of :func:`quantize_mx`: returns ``[payload, scales]``, both ``uint8``, ``[dim_x, dim_y // 2]`` (E2M1
+    codes, column 2j in the low half of byte j) and ``[dim_x, dim_y // 32]``; ``block_y`` is 32.  ``a`` is bfloat16 or
+    float32, its rows may lie apart (a slice of columns).  The scale is the largest power of two that keeps the group's
+    largest magnitude at or below 6; a group that holds an infinity or a NaN gets scale byte 255 (NaN).  No gradient."""
+    return _ops.quantize_mx_fp4.default(a, dim_x, dim_y, block_y)
+
+
+def dequantize_mx(payload: Tensor, scales: Tensor, dim_x: int, dim_y: int, block_y: int, elem_format: int,
+                  out_dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """The values ``decode(code) * 2 ** (scale - 127)`` that an MX matrix stands for, in bfloat16 or float32; NaN under a
+    scale byte of 255.  ``block_y``: a power of two from 8 to 256.  No gradient."""
+    return _ops.dequantize_mx.default(payload, scales, dim_x, dim_y, block_y, elem_format, out_dtype)
+
+
+def mx_matmul(a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, dim_m: int, dim_n: int, dim_k: int, a_format: int,
+              b_format: int, bias: Optional[Tensor] = None) -> Tensor:
+    """``A @ B.T (+ bias)`` of two MX matrices ``[dim_m, dim_k]`` and ``[dim_n, dim_k]`` with groups of 32 columns, as
+    bfloat16 ``[dim_m, dim_n]``: what a linear layer computes from quantised tokens and quantised weights, from one token
+    up.  Formats: both 4, or each 0 or 1.  Products and sums in binary32 on the block-scaled tensor core, one rounding at
+    the end; the same inputs give the same bits.  No gradient (see :func:`mx_matmul_grad` and ``mor_b200.nn.mx_linear``)."""
+    return _ops.mx_matmul.default(a, a_scales, b, b_scales, dim_m, dim_n, dim_k, a_format, b_format, bias)
+
+
+def mx_matmul_grad(g: Tensor, payload: Tensor, scales: Tensor, dim_m: int, dim_n: int, dim_k: int, elem_format: int,
+                   transpose_g: bool) -> Tensor:
+    """``g @ W`` (or ``g.T @ W`` with ``transpose_g``) as bfloat16 ``[dim_m, dim_n]``, for a bfloat16 ``g`` and an MX
+    matrix W ``[dim_k, dim_n]`` with groups of 32 columns, format 0, 1, 3 or 4: the input gradient of a linear layer from
+    its quantised weights, and its weight gradient from the quantised input that the forward pass kept."""
+    return _ops.mx_matmul_grad.default(g, payload, scales, dim_m, dim_n, dim_k, elem_format, transpose_g)
 
 
 # --------------------------------------------------------------------------- straight-through backward
