@@ -38,13 +38,6 @@ struct MmShape {
     static_assert(kSmem > 114 * 1024, "one CTA per SM");
 };
 
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int valid) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // Scale bytes of one row for one step: four a block, to the place the tensor core's copy takes them from (row r of 128:
 // 16 bytes for each r mod 32, four for each r / 32).  Rows and groups outside read as zero, a finite scale.
 template <int BLK>
@@ -295,6 +288,7 @@ int dispatch(const MxMatmulArgs& x, cudaStream_t st) {
     a.splits = 1;
     while (a.splits < 8 && tiles * a.splits * 2 <= sm_count() && a.ktiles >= a.splits * 4) a.splits *= 2;
     CUtensorMap mp, mq;
+    if (!bind_context()) return kErrLaunch;
     if (!make_swizzled_map(&mp, p, a.p_rows, row_bytes, row_bytes, 1, kPRows)) return kErrLaunch;
     if (!make_swizzled_map(&mq, q, a.q_rows, row_bytes, row_bytes, 1, tn)) return kErrLaunch;
     if (!swap) return go<FP4, 128, false>(mp, mq, a, tiles, st);

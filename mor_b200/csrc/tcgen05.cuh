@@ -133,6 +133,28 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t saddr, uint32_t rank) {
     return r;
 }
 
+// arrival on a barrier of another CTA of the cluster (its shared::cluster address), and the wait that pairs with it
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t remote) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {   // bounded, as mbar_wait_bounded
+    for (uint32_t spin = 0; spin < kSpinLimit; ++spin) {
+        uint32_t ok;
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+
+// four-byte asynchronous copies, zero-filled where `valid` is 0
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // two binary32 values to a packed bf16 word, round to nearest even (lo = the element at the lower address)
 __device__ __forceinline__ uint32_t pack_bf16_rne(float hi, float lo) {
     uint32_t r;
@@ -143,6 +165,13 @@ __device__ __forceinline__ uint32_t pack_bf16_rne(float hi, float lo) {
 // 2 ** (byte - 127), NaN for 255
 __device__ __forceinline__ float e8m0_to_f32(uint32_t byte) {
     return u2f(byte == 0 ? 0x00400000u : (byte == 255u ? 0x7FFFFFFFu : byte << 23));
+}
+
+// The encoder of tensor maps is a driver call and wants a context on the calling thread; a thread whose first CUDA call
+// this is (an autograd worker) has none until the runtime is told its device.
+inline bool bind_context() {
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
 }
 
 // row-major matrix of bytes (or bf16) with a row pitch, boxes of 128 bytes x box_rows under the 128-byte swizzle; what lies outside reads as zero

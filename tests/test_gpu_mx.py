@@ -226,6 +226,22 @@ def test_product_repeats_bit_for_bit_on_any_stream(m, n, k):
     assert all(torch.equal(first, o) for o in outs)
 
 
+def test_first_cuda_call_of_a_thread():
+    """a thread that has not touched the device before (autograd's workers) can make the calls"""
+    import threading
+    a, b, _ = product_case(130, 96, 256, E4M3, E4M3, 4, False)
+    args = [t.cuda() for t in (*a, *b)]
+    g = torch.randn(130, 96, device="cuda").to(torch.bfloat16)
+    calls = (lambda: ops().mx_matmul(*args, 130, 96, 256, 0, 0), lambda: ops().mx_matmul_grad(g, args[2], args[3], 130, 256, 96, 0, False))
+    for call in calls:
+        want, got = call(), []
+        t = threading.Thread(target=lambda: got.append(call()))
+        t.start()
+        t.join()
+        torch.cuda.synchronize()
+        assert got and torch.equal(got[0], want)
+
+
 def test_product_strided_and_offset_operands():
     a, b, _ = product_case(70, 96, 256, E4M3, E4M3, 4, False)
     want = ops().mx_matmul(*(t.cuda() for t in (*a, *b)), 70, 96, 256, 0, 0)
@@ -287,9 +303,32 @@ def test_grad_depths(k, fmt, across):
 
 @pytest.mark.parametrize("across", [False, True])
 @pytest.mark.parametrize("m,n,k,fmt", [(1000, 2080, 1500, E4M3), (2048, 1024, 4096, E2M1), (4096, 4096, 33, E4M3), (20, 64, 8192, E5M2),
-                                       (300, 32, 600, E4M3), (2500, 1056, 640, E2M1)])
+                                       (300, 32, 600, E4M3), (2500, 1056, 640, E2M1), (3000, 2080, 500, E4M3), (2304, 1312, 1000, E2M3),
+                                       (2568, 1312, 70, E5M2)])
 def test_grad_sizes(m, n, k, fmt, across):
     check_grad(m, n, k, fmt, across)
+
+
+@pytest.mark.parametrize("fmt", [E4M3, E5M2, E2M3, E2M1])
+def test_grad_extreme_scales_and_codes_that_are_no_number(fmt):
+    """scales down to 2^-127 make elements that are subnormal in bf16 (rounded there, half a step of 2^-133 at most), scales
+    up to 2^100 large ones; columns with an infinity or a NaN in them come out as such and the others do not"""
+    k, n, m = 96, 256, 64
+    gen = torch.Generator().manual_seed(2)
+    c, s = R.random_codes(k, n, fmt, 6)
+    s[:, 0::4], s[:, 1::4], s[:, 2::4] = 0, torch.randint(0, 12, (k, 2), generator=gen, dtype=torch.uint8), 227
+    if fmt in R.HAS_NAN:
+        c[3, 97], c[50, 130] = 0x7F, 0xFF
+        if fmt == E5M2:
+            c[4, 100], c[5, 140] = 0x7C, 0xFC
+    g = (torch.randint(1, 5, (m, k), generator=gen) * torch.where(torch.rand(m, k, generator=gen) < 0.5, -1, 1)).to(torch.bfloat16)
+    got = ops().mx_matmul_grad(g.cuda(), c.cuda(), s.cuda(), m, n, k, fmt, False).double().cpu()
+    w = R.decode(c, s, fmt)
+    exact = g.double() @ w
+    t = 2.0 ** -8 * exact.abs() + (math.ceil(k / 16) + 9) * 2.0 ** -23 * (g.abs().double() @ w.abs()) * 1.01 + k * 4 * 2.0 ** -134 + 2.0 ** -133
+    fine = torch.isfinite(exact)
+    assert torch.equal(torch.isnan(exact), torch.isnan(got)) and torch.equal(exact[~fine & ~torch.isnan(exact)], got[~fine & ~torch.isnan(exact)])
+    assert bool(((got - exact).abs()[fine] <= t[fine]).all())
 
 
 def test_grad_nan_scale_and_strides():
