@@ -4,9 +4,10 @@
 // multiplied into a product over k by the tensor core; the codes are widened to bf16 (exact: four significant bits at
 // most) on the way from the staged codes to the operand tile, which costs no global traffic beyond the codes.
 //
-// One kernel, persistent over output tiles.  Per step of 64 k a thread of warp 4 requests the gradient's tile and the
-// codes by TMA, warps 6-7 fetch the scale bytes, warps 8-15 widen the codes into the operand tile, a thread of warp 5
-// issues the products, and warps 0-3 write the tile before last while the next one accumulates (two accumulators).
+// One kernel, persistent over output tiles.  Per step of 64 k warp 4 requests the gradient's tile by TMA, warps 6-7 the
+// codes and their scale bytes, the widening warps turn the codes into the operand tile, warp 5 issues the products, and warps 0-3 write one tile by TMA while the next accumulates (two accumulators).  The
+// gradient's tiles, the codes and the widened tiles pass through rings of their own: codes are let go as soon as they are
+// in registers, and a widened tile is needed only briefly, so most of the shared memory covers the latency of loads.
 // In its large form two CTAs work as a pair on 256 x 256: each loads 128 rows of the gradient and widens 128 columns of W,
 // so every widened element meets 256 rows.
 #include <algorithm>
@@ -27,22 +28,41 @@ struct GrArgs {
 
 constexpr int kTK = 64;                 // k a step: 128 bytes of bf16
 constexpr int kABytes = 128 * kTK * 2;  // a CTA's rows of the gradient
-constexpr int kConvWarps = 8;
-constexpr int kThreads = 32 * (8 + kConvWarps);
+#ifndef KCW
+#define KCW 4
+#define KCG 2
+#endif
+constexpr int kConvWarps = KCW, kConvGroups = KCG;   // warps that widen a step together; the groups take the steps in turn
+constexpr int kThreads = 32 * (8 + kConvWarps * kConvGroups);
 
 template <int FMT, int CG, int NB>      // CTAs to a tile; columns of W that one CTA widens
 struct GrShape {
     static constexpr int kTM = 128 * CG, kTN = NB * CG;
     static constexpr int kRowBytes = FMT == kE2M1 ? NB / 2 : NB;   // codes of one k
     static constexpr int kBBytes = NB * kTK * 2;
-    static constexpr int kCodeBytes = kRowBytes * kTK;
-    static constexpr int kCodeOff = kABytes + kBBytes, kScaleOff = kCodeOff + kCodeBytes;
-    static constexpr int kStage = (kScaleOff + kTK * 4 + 1023) & ~1023;
-    static constexpr int kStages = (212 * 1024) / kStage;
-    static constexpr int kSmem = kStages * kStage + 1024;
+    static constexpr int kCodeBytes = kRowBytes * kTK, kCStage = kCodeBytes + kTK * 4;   // and their scale bytes
+#ifndef RA
+#define RA 4
+#define RB 4
+#define RC 6
+#endif
+    static constexpr int kSA = RA, kSB = RB, kSC = RC;                // depths of the rings
+    static constexpr int kBOff = kSA * kABytes, kCOff = kBOff + kSB * kBBytes;
+    static constexpr int kOutOff = kCOff + ((kSC * kCStage + 1023) & ~1023), kOutBytes = 128 * 128;   // two tiles of 128 x 64 on their way out
+    static constexpr int kSmem = kOutOff + 2 * kOutBytes + 1024;
     static constexpr int kCols = 2 * kTN;
     static_assert(kSmem > 114 * 1024, "one CTA per SM, so the columns of tensor memory suffice");
-    static_assert(kStages >= 4 && (kCols == 256 || kCols == 512), "shape");
+    static_assert(kSmem <= 227 * 1024 - 512 && (kCols == 256 || kCols == 512), "shape");
+};
+
+// a place in a ring of N slots and the parity of the round
+template <int N>
+struct Slot {
+    int s = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void advance(int by = 1) {
+        if ((s += by) >= N) { s -= N; phase ^= 1; }
+    }
 };
 
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
@@ -50,27 +70,19 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-// 2^(byte - 127) in both halves of a word, as bf16; NaN for 255
-__device__ __forceinline__ uint32_t e8m0_to_bf16x2(uint32_t byte) {
-    uint32_t b = byte << 7;
-    b = byte == 0 ? 0x0040u : b;
-    b = byte == 255u ? 0x7FFFu : b;
-    return b | (b << 16);
-}
-
 // Eight codes to eight bf16 values times the scale.  The exponent and mantissa of a code are the low bits of a bf16
 // pattern's: moved there, the pattern stands for the value times 2^-120 (E4M3; 2^-112, 2^-126 for the others), subnormal
-// codes included, since both formats count subnormals alike.  One multiplication undoes that exactly, a second
-// applies the scale with the only rounding there is.  Codes that are no finite number take the conversion instruction.
+// codes included, since both formats count subnormals alike.  One multiplication by 2^(scale - 127 + 120) undoes that and
+// applies the scale, with the only rounding there is.  It serves every scale whose product with 2^120 a bf16 holds and
+// every code that is a number; `odd` is set for the rest, which widen8_any takes.
 template <int FMT>
-__device__ __forceinline__ uint4 widen8(uint2 c, uint32_t scale2) {
+__device__ __forceinline__ uint4 widen8(uint2 c, uint32_t scale, uint32_t& odd) {
+    constexpr uint32_t lift = FMT == kE4M3 ? 120u : (FMT == kE5M2 ? 112u : 126u);
     uint32_t o[4];
     if constexpr (FMT == kE2M1) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {   // nibbles 2i, 2i + 1
-            const uint32_t x = (c.x >> (8 * i)) & 0xFu;
-            const uint32_t y = (c.x >> (8 * i + 4)) & 0xFu;
-            const uint32_t p = x | (y << 16);
+        for (int i = 0; i < 4; ++i) {   // nibbles 2i, 2i + 1 to the low ends of two halves
+            const uint32_t p = __byte_perm(c.x >> (8 * i), (c.x >> (8 * i)) >> 4, 0x0400) & 0x000F000Fu;
             o[i] = ((p << 12) & 0x80008000u) | ((p << 6) & 0x01C001C0u);
         }
     } else {
@@ -90,21 +102,29 @@ __device__ __forceinline__ uint4 widen8(uint2 c, uint32_t scale2) {
             }
         }
     }
-    constexpr uint32_t up = FMT == kE4M3 ? 0x7B807B80u : (FMT == kE5M2 ? 0x77807780u : 0x7E807E80u);   // 2^120, 2^112, 2^126
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = mul_bf16x2(o[i], up);
+    const uint32_t up = ((scale + lift) & 0xFFu) * 0x00800080u;
+    odd |= scale + lift > 254u ? 0x80u : 0u;
     if constexpr (FMT == kE4M3 || FMT == kE5M2) {
         constexpr uint32_t past = FMT == kE4M3 ? 0x01010101u : 0x04040404u;   // carries into bit 7 from 0x7F, from 0x7C up
-        if ((((c.x & 0x7F7F7F7Fu) + past) | ((c.y & 0x7F7F7F7Fu) + past)) & 0x80808080u) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t h2 = codes_to_h2<FMT>(((i < 2 ? c.x : c.y) >> (16 * (i & 1))) & 0xFFFFu);
-                o[i] = pack_bf16_rne(h_hi_to_f32(h2), h_lo_to_f32(h2));
-            }
-        }
+        odd |= ((c.x & 0x7F7F7F7Fu) + past) | ((c.y & 0x7F7F7F7Fu) + past);
     }
+    return make_uint4(mul_bf16x2(o[0], up), mul_bf16x2(o[1], up), mul_bf16x2(o[2], up), mul_bf16x2(o[3], up));
+}
+template <int FMT>
+__device__ __forceinline__ uint4 widen8_any(uint2 c, uint32_t scale) {
+    const float k = e8m0_to_f32(scale);
+    uint32_t o[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = mul_bf16x2(o[i], scale2);
+    for (int i = 0; i < 4; ++i) {
+        uint32_t h2;
+        if constexpr (FMT == kE2M1) {
+            const uint32_t b = (c.x >> (8 * i)) & 0xFFu;
+            asm("{\n.reg .b8 a, b, c, d;\nmov.b32 {a, b, c, d}, %1;\ncvt.rn.f16x2.e2m1x2 %0, a;\n}" : "=r"(h2) : "r"(b));
+        } else {
+            h2 = codes_to_h2<FMT>(((i < 2 ? c.x : c.y) >> (16 * (i & 1))) & 0xFFFFu);
+        }
+        o[i] = pack_bf16_rne(__fmul_rn(h_hi_to_f32(h2), k), __fmul_rn(h_lo_to_f32(h2), k));
+    }
     return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
@@ -120,16 +140,16 @@ __device__ __forceinline__ void tile_place(int t, int m_tiles, int n_tiles, int&
 
 template <int FMT, int CG, int NB>
 __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_c,
-                                                              const GrArgs a) {
+                                                              const __grid_constant__ CUtensorMap map_out, const GrArgs a) {
     using S = GrShape<FMT, CG, NB>;
-    constexpr int kLag = 3;
     extern __shared__ uint8_t s_raw[];
-    __shared__ __align__(8) uint64_t full[S::kStages], wide[S::kStages], empty[S::kStages], acc_full[2], acc_empty[2], drained;
+    __shared__ __align__(8) uint64_t full_a[S::kSA], empty_a[S::kSA], full_c[S::kSC], empty_c[S::kSC], wide[S::kSB], empty_b[S::kSB],
+        acc_full[2], acc_empty[2], drained;
     __shared__ uint32_t s_tmem;
     uint8_t* smem = s_raw + ((1024 - (smem_u32(s_raw) & 1023)) & 1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = CG == 2 ? (int)cluster_rank() : 0;
-    // work of this CTA (pair): tiles first, first + step, ... over steps [k_first, k_first + ksteps) of each
+    // work of this CTA (pair): tiles first, first + step, ... over steps [k_first, k_first + ks) of each
     const int split = CG == 2 ? 0 : (int)(blockIdx.x % (unsigned)a.splits);
     const int first = CG == 2 ? (int)(blockIdx.x >> 1) : (int)(blockIdx.x / (unsigned)a.splits);
     const int step = CG == 2 ? (int)(gridDim.x >> 1) : (int)(gridDim.x / (unsigned)a.splits);
@@ -137,11 +157,14 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
     const int ks = k_last - k_first;
 
     if (warp == 4 && lane == 0) {
-        for (int s = 0; s < S::kStages; ++s) { mbar_init(&full[s], 1 + 2); mbar_init(&wide[s], kConvWarps * CG); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < S::kSA; ++s) { mbar_init(&full_a[s], 1); mbar_init(&empty_a[s], 1); }
+        for (int s = 0; s < S::kSB; ++s) { mbar_init(&wide[s], kConvWarps * CG); mbar_init(&empty_b[s], 1); }
+        for (int s = 0; s < S::kSC; ++s) { mbar_init(&full_c[s], 1 + kTK); mbar_init(&empty_c[s], kConvWarps); }
         for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 4 * CG); }
         mbar_init(&drained, 1);
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_g));
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_c));
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_out));
     }
     if (warp == 5) tmem_alloc<CG>(&s_tmem, S::kCols);
     tc_fence_before();
@@ -151,89 +174,93 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
     pdl_launch_dependents();
     pdl_wait();
 
-    bool ok = true;   // a wait that ran out ends the role; what it would have computed is written as NaN
+    // A wait that ran out ends the role; what it would have computed is written as NaN.  A slot's first use finds its
+    // `empty` barrier in the phase before the first: waiting for the parity opposite to the round's passes at once.
+    bool ok = true;
     if (warp == 4) {
-        if (lane == 0) {
-            int i = 0;
-            for (int t = first; t < a.tiles && ok; t += step) {
-                int tm, tn;
-                tile_place(t, a.m_tiles, a.n_tiles, tm, tn);
-                const int m0 = tm * S::kTM + rank * 128, n0 = tn * S::kTN + rank * NB;
-                for (int j = 0; j < ks; ++j, ++i) {
-                    const int s = i % S::kStages;
-                    if (i >= S::kStages) ok = mbar_wait_bounded(&empty[s], (i / S::kStages - 1) & 1);
-                    if (!ok) break;
-                    uint8_t* st = smem + s * S::kStage;
+        Slot<S::kSA> sa;
+        for (int t = first; t < a.tiles && ok; t += step) {
+            int tm, tn;
+            tile_place(t, a.m_tiles, a.n_tiles, tm, tn);
+            const int m0 = tm * S::kTM + rank * 128;
+            for (int j = 0; j < ks; ++j) {
+                ok = mbar_wait_warp(&empty_a[sa.s], sa.phase ^ 1);
+                if (!ok) break;
+                if (elect_one()) {
                     const int k0 = (k_first + j) * kTK;
-                    mbar_expect_tx(&full[s], kABytes + S::kCodeBytes);
+                    uint8_t* as = smem + sa.s * kABytes;
+                    mbar_expect_tx(&full_a[sa.s], kABytes);
                     if (a.across) {   // g is [k, m]: two boxes of 64 m x 64 k
-                        tma_load_2d(st, &map_g, m0, k0, &full[s]);
-                        tma_load_2d(st + kABytes / 2, &map_g, m0 + 64, k0, &full[s]);
+                        tma_load_2d(as, &map_g, m0, k0, &full_a[sa.s]);
+                        tma_load_2d(as + kABytes / 2, &map_g, m0 + 64, k0, &full_a[sa.s]);
                     } else {
-                        tma_load_2d(st, &map_g, k0, m0, &full[s]);
+                        tma_load_2d(as, &map_g, k0, m0, &full_a[sa.s]);
                     }
-                    tma_load_2d(st + S::kCodeOff, &map_c, FMT == kE2M1 ? n0 / 2 : n0, k0, &full[s]);
                 }
+                __syncwarp();
+                sa.advance();
             }
-            if (!ok)   // copies in flight land before the shared memory is handed on
-                for (int j = i > S::kStages ? i - S::kStages : 0; j < i; ++j) mbar_wait_bounded(&full[j % S::kStages], (j / S::kStages) & 1);
         }
-        __syncwarp();
+        if (!ok)   // copies in flight land before the shared memory is handed on: every slot's last round
+            for (int s = 0; s < S::kSA; ++s) mbar_wait_bounded(&full_a[s], s < sa.s ? sa.phase : sa.phase ^ 1);
     } else if (warp == 5) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             const uint32_t idesc = idesc_bf16(S::kTM, S::kTN, a.across != 0, true);
             const uint32_t step_a = a.across ? 2048 / 16 : 32 / 16;
-            int i = 0, it = 0;
+            // operands whose rows run along m (n): 64 of them to a 128-byte row, such columns of tiles 8 KiB apart, eight k 1 KiB
+            const uint64_t da0 = a.across ? umma_desc(smem_u32(smem), 8192, 1024, kLayoutSwizzle128) : umma_desc_kmajor(smem_u32(smem));
+            const uint64_t db0 = umma_desc(smem_u32(smem + S::kBOff), 8192, 1024, kLayoutSwizzle128);
+            Slot<S::kSA> sa;
+            Slot<S::kSB> sb;
+            int it = 0;
             for (int t = first; t < a.tiles && ok; t += step, ++it) {
                 const int b = it & 1;
                 if (it >= 2) ok = mbar_wait_cluster(&acc_empty[b], (it / 2 - 1) & 1);
                 if (!ok) break;
-                tc_fence_after();
-                for (int j = 0; j < ks; ++j, ++i) {
-                    const int s = i % S::kStages;
-                    ok = mbar_wait_cluster(&wide[s], (i / S::kStages) & 1);
+                for (int j = 0; j < ks; ++j) {
+                    ok = mbar_wait_warp(&wide[sb.s], sb.phase);   // says that the gradient's tile is there too
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t st = smem_u32(smem + s * S::kStage);
-                    // operands whose rows run along m (n): 64 of them to a 128-byte row, such columns of tiles 8 KiB apart, eight k 1 KiB
-                    const uint64_t da = a.across ? umma_desc(st, 8192, 1024, kLayoutSwizzle128) : umma_desc_kmajor(st);
-                    const uint64_t db = umma_desc(st + kABytes, 8192, 1024, kLayoutSwizzle128);
+                    if (elect_one()) {
+                        const uint64_t da = da0 + sa.s * (kABytes / 16), db = db0 + sb.s * (S::kBBytes / 16);
 #pragma unroll
-                    for (int k = 0; k < kTK / 16; ++k)
-                        tc_mma_bf16<CG>(tmem + b * S::kTN, da + k * step_a, db + k * (2048 / 16), idesc, (j | k) != 0);
-                    if constexpr (CG == 2) tc_commit_pair(&empty[s]); else tc_commit(&empty[s]);
+                        for (int k = 0; k < kTK / 16; ++k)
+                            tc_mma_bf16<CG>(tmem + b * S::kTN, da + k * step_a, db + k * (2048 / 16), idesc, (j | k) != 0);
+                        if constexpr (CG == 2) { tc_commit_pair(&empty_b[sb.s]); tc_commit_pair(&empty_a[sa.s]); }
+                        else { tc_commit(&empty_b[sb.s]); tc_commit(&empty_a[sa.s]); }
+                        if (j == ks - 1) { if constexpr (CG == 2) tc_commit_pair(&acc_full[b]); else tc_commit(&acc_full[b]); }
+                    }
+                    __syncwarp();
+                    sa.advance();
+                    sb.advance();
                 }
-                if (!ok) break;
-                if constexpr (CG == 2) tc_commit_pair(&acc_full[b]); else tc_commit(&acc_full[b]);
             }
             if (!ok) {   // products in flight end before the tensor memory is handed on
-                if constexpr (CG == 2) tc_commit_pair(&drained); else tc_commit(&drained);
+                if (elect_one()) { if constexpr (CG == 2) tc_commit_pair(&drained); else tc_commit(&drained); }
+                __syncwarp();
                 mbar_wait_bounded(&drained, 0);
             }
         }
-        __syncwarp();
     } else if (warp == 6 || warp == 7) {
-        // scale bytes of one k each: four neighbouring groups
+        // codes, and the scale bytes of one k each: four neighbouring groups
         const int r = threadIdx.x - 192;
-        int i = 0, j = ks, t = first - step, grp = 0;
-        int64_t total = t < a.tiles && first < a.tiles ? (int64_t)((a.tiles - 1 - first) / step + 1) * ks : 0;
-        for (; i < total + kLag; ++i) {
-            if (i < total) {
-                if (j == ks) {
-                    j = 0;
-                    t += step;
-                    int tm, tn;
-                    tile_place(t, a.m_tiles, a.n_tiles, tm, tn);
-                    grp = tn * (S::kTN / 32) + (NB == 128 ? rank * 4 : 0);
-                }
-                const int s = i % S::kStages;
-                if (i >= S::kStages) ok = mbar_wait_bounded(&empty[s], (i / S::kStages - 1) & 1);
-                ok = __all_sync(0xFFFFFFFFu, ok);
+        Slot<S::kSC> sc;
+        for (int t = first; t < a.tiles && ok; t += step) {
+            int tm, tn;
+            tile_place(t, a.m_tiles, a.n_tiles, tm, tn);
+            const int n0 = tn * S::kTN + rank * NB, grp = n0 / 32;
+            for (int j = 0; j < ks; ++j) {
+                ok = mbar_wait_warp(&empty_c[sc.s], sc.phase ^ 1);
                 if (!ok) break;
+                if (warp == 6 && elect_one()) {
+                    mbar_expect_tx(&full_c[sc.s], S::kCodeBytes);
+                    tma_load_2d(smem + S::kCOff + sc.s * S::kCStage, &map_c, FMT == kE2M1 ? n0 / 2 : n0, (k_first + j) * kTK, &full_c[sc.s]);
+                }
+                __syncwarp();
                 const int64_t k = (int64_t)(k_first + j) * kTK + r;
                 const bool in = k < a.k && grp < a.groups;
                 const uint8_t* src = a.scales + (in ? k * a.groups + grp : 0);
-                const uint32_t dst = smem_u32(smem + s * S::kStage + S::kScaleOff) + 4 * r;
+                const uint32_t dst = smem_u32(smem + S::kCOff + sc.s * S::kCStage + S::kCodeBytes) + 4 * r;
                 if (a.fast_scales) {
                     cp_async4(dst, src, in ? 4 : 0);
                 } else {
@@ -245,86 +272,111 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
                     }
                     asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst), "r"(w) : "memory");
                 }
-                ++j;
-            }
-            cp_async_commit();
-            if (i >= kLag) {
-                cp_async_wait<kLag>();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&full[(i - kLag) % S::kStages]);
+                cp_async_arrive(&full_c[sc.s]);
+                sc.advance();
             }
         }
-        cp_async_wait<0>();
+        cp_async_wait_all();
+        if (!ok && warp == 6)
+            for (int s = 0; s < S::kSC; ++s) mbar_wait_bounded(&full_c[s], s < sc.s ? sc.phase : sc.phase ^ 1);
     } else if (warp >= 8) {
         // a lane owns eight neighbouring n of a row; eight lanes one 128-byte row of the operand tile
         constexpr int kLanesPerRow = NB / 8, kRowsPerPass = 32 * kConvWarps / kLanesPerRow, kPasses = kTK / kRowsPerPass;
-        const int ct = threadIdx.x - 256, u = ct & 7, nc = (ct / 8) % (NB / 64), r0 = ct / kLanesPerRow;
-        const uint32_t wide0 = CG == 2 ? map_to_rank(smem_u32(&wide[0]), 0) : smem_u32(&wide[0]);
-        const int sbyte = nc * 2 + (u >> 2) + (NB == 64 ? rank * 2 : 0);
+        const int ct = (threadIdx.x - 256) % (32 * kConvWarps), group = (warp - 8) / kConvWarps, u = ct & 7, nc = (ct / 8) % (NB / 64), r0 = ct / kLanesPerRow;
+        const uint32_t wide0 = CG == 2 ? map_to_rank(smem_u32(&wide[0]), 0) : smem_u32(&wide[0]);   // the pair's issuer waits for both halves
+        const int sbyte = nc * 2 + (u >> 2);
         const int64_t total = first < a.tiles ? (int64_t)((a.tiles - 1 - first) / step + 1) * ks : 0;
-        for (int64_t i = 0; i < total; ++i) {
-            const int s = (int)(i % S::kStages);
-            ok = mbar_wait_bounded(&full[s], (uint32_t)(i / S::kStages) & 1);
-            ok = __all_sync(0xFFFFFFFFu, ok);
+        Slot<S::kSA> sa;
+        Slot<S::kSB> sb;
+        Slot<S::kSC> sc;
+        sa.s = sb.s = sc.s = group;
+        for (int64_t i = group; i < total; i += kConvGroups) {
+            ok = mbar_wait_warp(&full_c[sc.s], sc.phase);
             if (!ok) break;
-            uint8_t* st = smem + s * S::kStage;
+            const uint8_t* cs = smem + S::kCOff + sc.s * S::kCStage;
             uint2 c[kPasses];
-            uint32_t sb[kPasses];
+            uint32_t k8[kPasses], odd = 0;
 #pragma unroll
             for (int p = 0; p < kPasses; ++p) {
                 const int row = r0 + p * kRowsPerPass;
-                const uint8_t* codes = st + S::kCodeOff + row * S::kRowBytes;
-                if constexpr (FMT == kE2M1) c[p] = make_uint2(*reinterpret_cast<const uint32_t*>(codes + nc * 32 + u * 4), 0u);
-                else c[p] = *reinterpret_cast<const uint2*>(codes + nc * 64 + u * 8);
-                sb[p] = st[S::kScaleOff + 4 * row + sbyte];
+                if constexpr (FMT == kE2M1) c[p] = make_uint2(*reinterpret_cast<const uint32_t*>(cs + row * S::kRowBytes + nc * 32 + u * 4), 0u);
+                else c[p] = *reinterpret_cast<const uint2*>(cs + row * S::kRowBytes + nc * 64 + u * 8);
+                k8[p] = cs[S::kCodeBytes + 4 * row + sbyte];
             }
+            __syncwarp();
+            if (elect_one()) mbar_arrive(&empty_c[sc.s]);
+            ok = mbar_wait_warp(&empty_b[sb.s], sb.phase ^ 1);
+            if (!ok) break;
+            uint8_t* bs = smem + S::kBOff + sb.s * S::kBBytes + nc * 8192 + r0 * 128;
 #pragma unroll
-            for (int p = 0; p < kPasses; ++p) {
-                const int row = r0 + p * kRowsPerPass;
-                *reinterpret_cast<uint4*>(st + kABytes + nc * 8192 + row * 128 + ((u ^ (row & 7)) << 4)) = widen8<FMT>(c[p], e8m0_to_bf16x2(sb[p]));
+            for (int p = 0; p < kPasses; ++p)   // passes are a multiple of eight rows apart: the same swizzle
+                *reinterpret_cast<uint4*>(bs + p * (kRowsPerPass * 128) + ((u ^ (r0 & 7)) << 4)) = widen8<FMT>(c[p], k8[p], odd);
+            if (odd & 0x80808080u) {
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p)
+                    *reinterpret_cast<uint4*>(bs + p * (kRowsPerPass * 128) + ((u ^ (r0 & 7)) << 4)) = widen8_any<FMT>(c[p], k8[p]);
             }
             fence_async_shared();
+            if (ct < 32) ok = mbar_wait_warp(&full_a[sa.s], sa.phase);   // one warp's arrival vouches for the gradient's tile
+            if (!ok) break;
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(wide0 + 8 * s);
+            if (elect_one()) mbar_arrive_peer(wide0 + 8 * sb.s);
+            sa.advance(kConvGroups);
+            sb.advance(kConvGroups);
+            sc.advance(kConvGroups);
         }
+        static_assert(kRowsPerPass % 8 == 0, "swizzle");
     } else {
         int it = 0;
         const uint32_t empty0 = CG == 2 ? map_to_rank(smem_u32(&acc_empty[0]), 0) : smem_u32(&acc_empty[0]);
+        int ob = 0;
         for (int t = first; t < a.tiles; t += step, ++it) {
             int tm, tn;
             tile_place(t, a.m_tiles, a.n_tiles, tm, tn);
-            const int64_t m = (int64_t)tm * S::kTM + rank * 128 + threadIdx.x, n0 = (int64_t)tn * S::kTN;
+            const int m0 = tm * S::kTM + rank * 128, n0 = tn * S::kTN;
             const int b = it & 1;
-            ok = ok && mbar_wait_bounded(&acc_full[b], (it / 2) & 1);
-            ok = __all_sync(0xFFFFFFFFu, ok);
+            ok = ok && mbar_wait_warp(&acc_full[b], (it / 2) & 1);
             tc_fence_after();
             const uint32_t acc = tmem + b * S::kTN + ((uint32_t)warp << 21);
 #pragma unroll 1
-            for (int c0 = 0; c0 < S::kTN; c0 += 32) {
-                uint32_t r[32];
-                tmem_load32(acc + c0, r);
+            for (int c0 = 0; c0 < S::kTN; c0 += 64) {
+                uint32_t r[2][32];
+                tmem_load32(acc + c0, r[0]);
+                tmem_load32(acc + c0 + 32, r[1]);
                 tmem_wait_loads();
                 if (!ok) {
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) r[c] = 0x7FFFFFFFu;
+                    for (int c = 0; c < 32; ++c) r[0][c] = r[1][c] = 0x7FFFFFFFu;
                 }
                 if (a.splits > 1) {
                     float* part = reinterpret_cast<float*>(smem);   // [column][128 rows]; the operands are no longer needed
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) part[(c0 + c) * 128 + threadIdx.x] = u2f(r[c]);
-                } else if (m < a.m && n0 + c0 < a.n) {   // n is a multiple of 32
-                    uint16_t* o = a.out + m * a.n + n0 + c0;
+                    for (int c = 0; c < 64; ++c) part[(c0 + c) * 128 + threadIdx.x] = u2f(r[c >> 5][c & 31]);
+                } else {
+                    uint8_t* os = smem + S::kOutOff + ob * S::kOutBytes;
+                    if (threadIdx.x == 0) bulk_wait_reads_but<1>();   // the store from this buffer before last has read it
+                    named_barrier(1, 128);
 #pragma unroll
-                    for (int c = 0; c < 32; c += 8)
-                        *reinterpret_cast<uint4*>(o + c) = make_uint4(
-                            pack_bf16_rne(u2f(r[c + 1]), u2f(r[c])), pack_bf16_rne(u2f(r[c + 3]), u2f(r[c + 2])),
-                            pack_bf16_rne(u2f(r[c + 5]), u2f(r[c + 4])), pack_bf16_rne(u2f(r[c + 7]), u2f(r[c + 6])));
+                    for (int c = 0; c < 8; ++c) {
+                        const uint32_t* q = &r[c >> 2][(c & 3) * 8];
+                        *reinterpret_cast<uint4*>(os + threadIdx.x * 128 + ((c ^ (threadIdx.x & 7)) << 4)) =
+                            make_uint4(pack_bf16_rne(u2f(q[1]), u2f(q[0])), pack_bf16_rne(u2f(q[3]), u2f(q[2])), pack_bf16_rne(u2f(q[5]), u2f(q[4])),
+                                       pack_bf16_rne(u2f(q[7]), u2f(q[6])));
+                    }
+                    fence_async_shared();
+                    named_barrier(1, 128);
+                    if (threadIdx.x == 0) {
+                        if (m0 < a.m && n0 + c0 < a.n) tma_store_2d(&map_out, os, n0 + c0, m0);
+                        bulk_commit();
+                    }
+                    ob ^= 1;
                 }
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(empty0 + 8 * b);
+            if (elect_one()) mbar_arrive_cluster(empty0 + 8 * b);
         }
+        if (threadIdx.x == 0) bulk_wait_reads();
     }
 
     if (CG == 1 && a.splits > 1) {   // partial sums of one tile in the CTAs of a cluster: each adds up some of the columns, in rank order
@@ -395,9 +447,10 @@ int go(const MxGradArgs& x, cudaStream_t st) {
         while (a.splits < 8 && a.tiles * a.splits * 2 <= sm_count() && a.ksteps >= a.splits * 4) a.splits *= 2;
         grid = a.splits > 1 ? a.tiles * a.splits : std::min(a.tiles, sm_count());
     }
-    CUtensorMap mg, mc;
+    CUtensorMap mg, mc, mo;
     const bool made = x.across ? make_swizzled_map(&mg, x.g, x.k, x.m, x.g_pitch * 2, 2, kTK) : make_swizzled_map(&mg, x.g, x.m, x.k, x.g_pitch * 2, 2, 128);
     if (!made || !make_code_map(&mc, x.payload, x.k, FMT == kE2M1 ? x.n / 2 : x.n, S::kRowBytes, kTK)) return kErrLaunch;
+    if (!make_swizzled_map(&mo, x.out, x.m, x.n, x.n * 2, 2, 128)) return kErrLaunch;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kThreads);
@@ -410,7 +463,7 @@ int go(const MxGradArgs& x, cudaStream_t st) {
     attr[1].val.clusterDim = {(unsigned)(CG == 2 ? 2 : a.splits), 1, 1};
     cfg.attrs = attr;
     cfg.numAttrs = CG == 2 || a.splits > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kern, mg, mc, a) == cudaSuccess ? check_launch() : kErrLaunch;
+    return cudaLaunchKernelEx(&cfg, kern, mg, mc, mo, a) == cudaSuccess ? check_launch() : kErrLaunch;
 }
 
 // Pairs where the 256 x 256 tiles fill at least half of the pairs' slots in the last round; single CTAs on 128 x 128, with the sum over

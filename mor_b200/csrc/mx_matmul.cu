@@ -66,7 +66,6 @@ template <bool FP4, int TN, bool SWAP>
 __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                                                            const MmArgs a) {
     using S = MmShape<FP4, TN>;
-    constexpr int kLag = S::kStages - 1 < 4 ? S::kStages - 1 : 4;
     constexpr int kGroupsPerStep = FP4 ? 8 : 4;
     extern __shared__ uint8_t s_raw[];
     __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], acc_done, drained;
@@ -81,7 +80,7 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
     const int n = k_last - k_first;
 
     if (warp == 4 && lane == 0) {
-        for (int s = 0; s < S::kStages; ++s) { mbar_init(&full[s], 1 + 4); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(&full[s], 1 + 128); mbar_init(&empty[s], 1); }
         mbar_init(&acc_done, 1);
         mbar_init(&drained, 1);
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_p));
@@ -119,6 +118,7 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
                 const int s = i % S::kStages;
                 ok = mbar_wait_bounded(&full[s], (i / S::kStages) & 1);
                 if (!ok) break;
+                fence_async_shared();   // the scale bytes came by ordinary copies, the tensor core reads them through its own path
                 tc_fence_after();
                 const uint32_t st = smem_u32(smem + s * S::kStage);
                 const uint32_t sfp = tmem + TN + (i & 1) * S::kSfCols, sfq = sfp + 4 * S::kBlk;
@@ -140,29 +140,21 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
     } else {
         const int t = threadIdx.x;   // 0..127
         const uint32_t place = (t & 31) * 16 + (t >> 5) * 4;
-        for (int i = 0; i < n + kLag; ++i) {
-            if (i < n) {
-                const int s = i % S::kStages;
-                if (i >= S::kStages) ok = mbar_wait_bounded(&empty[s], (i / S::kStages - 1) & 1);
-                ok = __all_sync(0xFFFFFFFFu, ok);
-                if (!ok) break;
-                const uint32_t sf = smem_u32(smem + s * S::kStage + S::kSfOff) + place;
-                const int64_t g0 = (int64_t)(k_first + i) * kGroupsPerStep;
-                load_scales<S::kBlk>(sf, a.sp, p0 + t, a.p_rows, a.groups, g0, a.fast_scales);
+        for (int i = 0; i < n; ++i) {
+            const int s = i % S::kStages;
+            if (i >= S::kStages) ok = mbar_wait_bounded(&empty[s], (i / S::kStages - 1) & 1);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            const uint32_t sf = smem_u32(smem + s * S::kStage + S::kSfOff) + place;
+            const int64_t g0 = (int64_t)(k_first + i) * kGroupsPerStep;
+            load_scales<S::kBlk>(sf, a.sp, p0 + t, a.p_rows, a.groups, g0, a.fast_scales);
 #pragma unroll
-                for (int h = 0; h < (TN + 127) / 128; ++h)
-                    if (h * 128 + t < TN)
-                        load_scales<S::kBlk>(sf + 512 * (S::kBlk + h), a.sq, q0 + h * 128 + t, a.q_rows, a.groups, g0, a.fast_scales);
-            }
-            cp_async_commit();
-            if (i >= kLag) {
-                cp_async_wait<kLag>();
-                fence_async_shared();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&full[(i - kLag) % S::kStages]);
-            }
+            for (int h = 0; h < (TN + 127) / 128; ++h)
+                if (h * 128 + t < TN)
+                    load_scales<S::kBlk>(sf + 512 * (S::kBlk + h), a.sq, q0 + h * 128 + t, a.q_rows, a.groups, g0, a.fast_scales);
+            cp_async_arrive(&full[s]);
         }
-        cp_async_wait<0>();
+        cp_async_wait_all();
         ok = ok && mbar_wait_bounded(&acc_done, 0);
         ok = __all_sync(0xFFFFFFFFu, ok);
         tc_fence_after();

@@ -122,6 +122,15 @@ __device__ __forceinline__ void tmem_load16(uint32_t taddr, uint32_t (&r)[16]) {
 }
 __device__ __forceinline__ void tmem_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// a tile of shared memory to global memory under the map's swizzle; what lies outside the tensor is not written
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(smem_u32(src)) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void bulk_wait_reads_but() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+// a barrier of some warps of the CTA
+__device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
 // clusters
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ void cluster_sync() {
@@ -137,23 +146,44 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t saddr, uint32_t rank) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t remote) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
 }
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {   // bounded, as mbar_wait_bounded
+// The same without a fence to the cluster's scope, which takes about 0.9 us: for a CTA that vouches for what lies in its
+// own shared memory and is read there, by its own SM's tensor core, after the writers' proxy fences.
+__device__ __forceinline__ void mbar_arrive_peer(uint32_t remote) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {   // bounded, by a whole warp
+    bool done = false;
     for (uint32_t spin = 0; spin < kSpinLimit; ++spin) {
         uint32_t ok;
         asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
                      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-        if (ok) return true;
+        if (ok) { done = true; break; }
     }
-    return false;
+    return __all_sync(0xFFFFFFFFu, done) != 0;
+}
+
+// One lane of a converged warp.  The roles of a product kernel run as whole warps, every lane waiting on the barriers, and
+// only what is issued once is issued by the elected lane: a wait in a branch of one lane takes 190 cycles even when it is
+// over before it begins, one of a whole warp 90.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
+}
+// a whole warp waits, and all its lanes learn alike whether the wait ran out
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar, parity)) != 0;
 }
 
 // four-byte asynchronous copies, zero-filled where `valid` is 0
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int valid) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// one arrival on the barrier when all such copies of this thread so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // two binary32 values to a packed bf16 word, round to nearest even (lo = the element at the lower address)
 __device__ __forceinline__ uint32_t pack_bf16_rne(float hi, float lo) {
