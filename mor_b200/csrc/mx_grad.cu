@@ -4,8 +4,8 @@
 // multiplied into a product over k by the tensor core; the codes are widened to bf16 (exact: four significant bits at
 // most) on the way from the staged codes to the operand tile, which costs no global traffic beyond the codes.
 //
-// One kernel, persistent over output tiles.  Per step of 64 k warp 4 requests the gradient's tile by TMA, warps 6-7 the
-// codes and their scale bytes, the widening warps turn the codes into the operand tile, warp 5 issues the products, and warps 0-3 write one tile by TMA while the next accumulates (two accumulators).  The
+// One kernel, persistent over output tiles.  Per step of 64 k warp 4 requests the gradient's tile by TMA, warp 6 the
+// codes, warps 7-8 their scale bytes, the widening warps turn the codes into the operand tile, warp 5 issues the products, and warps 0-3 write one tile by TMA while the next accumulates (two accumulators).  The
 // gradient's tiles, the codes and the widened tiles pass through rings of their own: codes are let go as soon as they are
 // in registers, and a widened tile is needed only briefly, so most of the shared memory covers the latency of loads.
 // In its large form two CTAs work as a pair on 256 x 256: each loads 128 rows of the gradient and widens 128 columns of W,
@@ -28,12 +28,9 @@ struct GrArgs {
 
 constexpr int kTK = 64;                 // k a step: 128 bytes of bf16
 constexpr int kABytes = 128 * kTK * 2;  // a CTA's rows of the gradient
-#ifndef KCW
-#define KCW 4
-#define KCG 2
-#endif
-constexpr int kConvWarps = KCW, kConvGroups = KCG;   // warps that widen a step together; the groups take the steps in turn
-constexpr int kThreads = 32 * (8 + kConvWarps * kConvGroups);
+constexpr int kConvWarps = 4, kConvGroups = 3;   // warps that widen a step together; the groups take the steps in turn
+constexpr int kFirstConv = 9;                    // warps 0-3 write, 4 gradient, 5 products, 6 codes, 7-8 scales
+constexpr int kThreads = 32 * (kFirstConv + kConvWarps * kConvGroups);
 
 template <int FMT, int CG, int NB>      // CTAs to a tile; columns of W that one CTA widens
 struct GrShape {
@@ -41,12 +38,7 @@ struct GrShape {
     static constexpr int kRowBytes = FMT == kE2M1 ? NB / 2 : NB;   // codes of one k
     static constexpr int kBBytes = NB * kTK * 2;
     static constexpr int kCodeBytes = kRowBytes * kTK, kCStage = kCodeBytes + kTK * 4;   // and their scale bytes
-#ifndef RA
-#define RA 4
-#define RB 4
-#define RC 6
-#endif
-    static constexpr int kSA = RA, kSB = RB, kSC = RC;                // depths of the rings
+    static constexpr int kSA = 4, kSB = 4, kSC = 5;                // depths of the rings
     static constexpr int kBOff = kSA * kABytes, kCOff = kBOff + kSB * kBBytes;
     static constexpr int kOutOff = kCOff + ((kSC * kCStage + 1023) & ~1023), kOutBytes = 128 * 128;   // two tiles of 128 x 64 on their way out
     static constexpr int kSmem = kOutOff + 2 * kOutBytes + 1024;
@@ -241,31 +233,46 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
                 mbar_wait_bounded(&drained, 0);
             }
         }
-    } else if (warp == 6 || warp == 7) {
-        // codes, and the scale bytes of one k each: four neighbouring groups
-        const int r = threadIdx.x - 192;
+    } else if (warp == 6) {
         Slot<S::kSC> sc;
         for (int t = first; t < a.tiles && ok; t += step) {
             int tm, tn;
             tile_place(t, a.m_tiles, a.n_tiles, tm, tn);
-            const int n0 = tn * S::kTN + rank * NB, grp = n0 / 32;
+            const int n0 = tn * S::kTN + rank * NB;
             for (int j = 0; j < ks; ++j) {
                 ok = mbar_wait_warp(&empty_c[sc.s], sc.phase ^ 1);
                 if (!ok) break;
-                if (warp == 6 && elect_one()) {
+                if (elect_one()) {
                     mbar_expect_tx(&full_c[sc.s], S::kCodeBytes);
                     tma_load_2d(smem + S::kCOff + sc.s * S::kCStage, &map_c, FMT == kE2M1 ? n0 / 2 : n0, (k_first + j) * kTK, &full_c[sc.s]);
                 }
                 __syncwarp();
-                const int64_t k = (int64_t)(k_first + j) * kTK + r;
-                const bool in = k < a.k && grp < a.groups;
-                const uint8_t* src = a.scales + (in ? k * a.groups + grp : 0);
-                const uint32_t dst = smem_u32(smem + S::kCOff + sc.s * S::kCStage + S::kCodeBytes) + 4 * r;
+                sc.advance();
+            }
+        }
+        if (!ok)
+            for (int s = 0; s < S::kSC; ++s) mbar_wait_bounded(&full_c[s], s < sc.s ? sc.phase : sc.phase ^ 1);
+    } else if (warp == 7 || warp == 8) {
+        // scale bytes of one k to a lane: four neighbouring groups
+        const int r = threadIdx.x - 7 * 32;
+        const uint32_t dst0 = smem_u32(smem + S::kCOff + S::kCodeBytes) + 4 * r;
+        const int64_t stride = (int64_t)kTK * a.groups;
+        Slot<S::kSC> sc;
+        for (int t = first; t < a.tiles && ok; t += step) {
+            int tm, tn;
+            tile_place(t, a.m_tiles, a.n_tiles, tm, tn);
+            const int grp = (tn * S::kTN + rank * NB) / 32;
+            int64_t left = grp < a.groups ? a.k - (int64_t)k_first * kTK - r : 0;   // this lane's k is inside while positive
+            const uint8_t* src = a.scales + ((int64_t)k_first * kTK + r) * a.groups + grp;
+            for (int j = 0; j < ks; ++j) {
+                ok = mbar_wait_warp(&empty_c[sc.s], sc.phase ^ 1);
+                if (!ok) break;
+                const uint32_t dst = dst0 + sc.s * S::kCStage;
                 if (a.fast_scales) {
-                    cp_async4(dst, src, in ? 4 : 0);
+                    cp_async4(dst, left > 0 ? src : a.scales, left > 0 ? 4 : 0);
                 } else {
                     uint32_t w = 0;
-                    if (in) {
+                    if (left > 0) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             if (grp + e < a.groups) w |= (uint32_t)__ldg(src + e) << (8 * e);
@@ -274,15 +281,15 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
                 }
                 cp_async_arrive(&full_c[sc.s]);
                 sc.advance();
+                src += stride;
+                left -= kTK;
             }
         }
         cp_async_wait_all();
-        if (!ok && warp == 6)
-            for (int s = 0; s < S::kSC; ++s) mbar_wait_bounded(&full_c[s], s < sc.s ? sc.phase : sc.phase ^ 1);
-    } else if (warp >= 8) {
+    } else if (warp >= kFirstConv) {
         // a lane owns eight neighbouring n of a row; eight lanes one 128-byte row of the operand tile
         constexpr int kLanesPerRow = NB / 8, kRowsPerPass = 32 * kConvWarps / kLanesPerRow, kPasses = kTK / kRowsPerPass;
-        const int ct = (threadIdx.x - 256) % (32 * kConvWarps), group = (warp - 8) / kConvWarps, u = ct & 7, nc = (ct / 8) % (NB / 64), r0 = ct / kLanesPerRow;
+        const int ct = (threadIdx.x - 32 * kFirstConv) % (32 * kConvWarps), group = (warp - kFirstConv) / kConvWarps, u = ct & 7, nc = (ct / 8) % (NB / 64), r0 = ct / kLanesPerRow;
         const uint32_t wide0 = CG == 2 ? map_to_rank(smem_u32(&wide[0]), 0) : smem_u32(&wide[0]);   // the pair's issuer waits for both halves
         const int sbyte = nc * 2 + (u >> 2);
         const int64_t total = first < a.tiles ? (int64_t)((a.tiles - 1 - first) / step + 1) * ks : 0;
@@ -307,14 +314,13 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
             if (elect_one()) mbar_arrive(&empty_c[sc.s]);
             ok = mbar_wait_warp(&empty_b[sb.s], sb.phase ^ 1);
             if (!ok) break;
-            uint8_t* bs = smem + S::kBOff + sb.s * S::kBBytes + nc * 8192 + r0 * 128;
+            uint8_t* bs = smem + S::kBOff + sb.s * S::kBBytes + nc * 8192 + r0 * 128 + ((u ^ (r0 & 7)) << 4);
 #pragma unroll
             for (int p = 0; p < kPasses; ++p)   // passes are a multiple of eight rows apart: the same swizzle
-                *reinterpret_cast<uint4*>(bs + p * (kRowsPerPass * 128) + ((u ^ (r0 & 7)) << 4)) = widen8<FMT>(c[p], k8[p], odd);
+                *reinterpret_cast<uint4*>(bs + p * (kRowsPerPass * 128)) = widen8<FMT>(c[p], k8[p], odd);
             if (odd & 0x80808080u) {
 #pragma unroll
-                for (int p = 0; p < kPasses; ++p)
-                    *reinterpret_cast<uint4*>(bs + p * (kRowsPerPass * 128) + ((u ^ (r0 & 7)) << 4)) = widen8_any<FMT>(c[p], k8[p]);
+                for (int p = 0; p < kPasses; ++p) *reinterpret_cast<uint4*>(bs + p * (kRowsPerPass * 128)) = widen8_any<FMT>(c[p], k8[p]);
             }
             fence_async_shared();
             if (ct < 32) ok = mbar_wait_warp(&full_a[sa.s], sa.phase);   // one warp's arrival vouches for the gradient's tile
@@ -325,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
             sb.advance(kConvGroups);
             sc.advance(kConvGroups);
         }
-        static_assert(kRowsPerPass % 8 == 0, "swizzle");
+        static_assert(kRowsPerPass % 8 == 0 && kConvGroups <= S::kSA && kConvGroups <= S::kSB && kConvGroups <= S::kSC, "swizzle, first slots");
     } else {
         int it = 0;
         const uint32_t empty0 = CG == 2 ? map_to_rank(smem_u32(&acc_empty[0]), 0) : smem_u32(&acc_empty[0]);
