@@ -7,9 +7,8 @@
  *   scales:  one E8M0 byte for every `block_cols` consecutive columns of a row, row-major;
  *   element = decode(code) * 2^(scale - 127), NaN where the scale byte is 255.
  * All pointers are device pointers of the current device; tensors are row-major and, unless said otherwise, contiguous.
- * Calls enqueue on `stream`, do not synchronise, allocate or throw, need no workspace, and may be captured into a CUDA
- * graph.  Status codes are those of mor_b200.h (0 ok, -1 invalid argument, -2 unsupported shape or alignment, -4 launch
- * failed, -5 too large).  Sizes of zero in rows, m or n are valid and launch nothing.
+ * Calls enqueue on `stream`, do not synchronise, allocate or throw, and may be captured into a CUDA graph.  Status codes are those of mor_b200.h (0 ok, -1 invalid argument, -2 unsupported shape or alignment, -3
+ * workspace missing or too small, -4 launch failed, -5 too large).  Sizes of zero in rows, m or n are valid and launch nothing.
  * A tile of a product whose operands did not arrive within the kernel's bounded wait is written as NaN. */
 #ifndef MOR_B200_MX_H
 #define MOR_B200_MX_H
@@ -48,10 +47,13 @@ MOR_B200_MX_API int mor_b200_mx_dequantize(const void* payload, const void* scal
  * 16-byte aligned.  Formats: both E2M1, or each E4M3 or E5M2.  bias: bf16 [n] or NULL; out: bf16 [m, n].  Products
  * and sums are formed by the tensor core in binary32, the result (bias added in binary32) is rounded once.  m <= 64 takes a form in which
  * tokens fill a narrow tile; sums split over the CTAs of a cluster are added in a fixed order, so results repeat
- * bit for bit. */
+ * bit for bit.  Large products need a workspace of mor_b200_mx_matmul_workspace_bytes(m, n, k) bytes (0 for the others,
+ * which take NULL), 16-byte aligned; the scale bytes lie in it in tensor-core order while the call runs, so calls that
+ * may overlap (other streams, captured graphs) need one each. */
+MOR_B200_MX_API size_t mor_b200_mx_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k);
 MOR_B200_MX_API int mor_b200_mx_matmul(const void* a, const void* a_scales, const void* b, const void* b_scales, int64_t m,
                                        int64_t n, int64_t k, int a_format, int b_format, const void* bias, void* out,
-                                       void* stream);
+                                       void* workspace, size_t workspace_bytes, void* stream);
 
 /* out[m, n] = sum_k op(g)[m, k] W[k, n]: g is bf16 [m, k], or [k, m] with transpose_g, `g_pitch` elements from row to
  * row (g 16-byte aligned, g_pitch a multiple of 8); W is MX [k, n] with groups of 32 along n, n a multiple of 32, format

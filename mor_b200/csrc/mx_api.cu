@@ -43,8 +43,13 @@ int mor_b200_mx_dequantize(const void* payload, const void* scales, void* out, i
                              static_cast<cudaStream_t>(stream));
 }
 
+size_t mor_b200_mx_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+    if (m <= 0 || n <= 0 || k <= 0 || k % 32 || too_large(m) || too_large(n) || too_large(k)) return 0;
+    return mx_matmul_workspace(m, n, k);
+}
+
 int mor_b200_mx_matmul(const void* a, const void* a_scales, const void* b, const void* b_scales, int64_t m, int64_t n, int64_t k,
-                       int a_format, int b_format, const void* bias, void* out, void* stream) {
+                       int a_format, int b_format, const void* bias, void* out, void* workspace, size_t workspace_bytes, void* stream) {
     if (m < 0 || n < 0 || k <= 0) return kErrInvalidArgument;
     const bool fp4 = a_format == kE2M1 && b_format == kE2M1;
     const bool fp8 = (a_format == kE4M3 || a_format == kE5M2) && (b_format == kE4M3 || b_format == kE5M2);
@@ -54,7 +59,9 @@ int mor_b200_mx_matmul(const void* a, const void* a_scales, const void* b, const
     if (!a || !a_scales || !b || !b_scales || !out) return kErrInvalidArgument;
     if (too_large(m) || too_large(n) || too_large(k)) return kErrTooLarge;
     if (!aligned(a, 16) || !aligned(b, 16) || !aligned(out, 2) || !aligned(bias, 2)) return kErrUnsupportedShape;
-    const MxMatmulArgs x{a, b, static_cast<const uint8_t*>(a_scales), static_cast<const uint8_t*>(b_scales), bias, out, m, n, k, a_format, b_format};
+    const size_t need = mx_matmul_workspace(m, n, k);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return kErrWorkspace;
+    const MxMatmulArgs x{a, b, static_cast<const uint8_t*>(a_scales), static_cast<const uint8_t*>(b_scales), bias, out, m, n, k, a_format, b_format, workspace};
     return launch_mx_matmul(x, static_cast<cudaStream_t>(stream));
 }
 

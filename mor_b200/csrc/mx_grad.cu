@@ -47,16 +47,6 @@ struct GrShape {
     static_assert(kSmem <= 227 * 1024 - 512 && (kCols == 256 || kCols == 512), "shape");
 };
 
-// a place in a ring of N slots and the parity of the round
-template <int N>
-struct Slot {
-    int s = 0;
-    uint32_t phase = 0;
-    __device__ __forceinline__ void advance(int by = 1) {
-        if ((s += by) >= N) { s -= N; phase ^= 1; }
-    }
-};
-
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -118,16 +108,6 @@ __device__ __forceinline__ uint4 widen8_any(uint2 c, uint32_t scale) {
         o[i] = pack_bf16_rne(__fmul_rn(h_hi_to_f32(h2), k), __fmul_rn(h_lo_to_f32(h2), k));
     }
     return make_uint4(o[0], o[1], o[2], o[3]);
-}
-
-// Output tile number -> its place: bands of eight rows of tiles, down a band's columns, so that the CTAs at work at one
-// time share rows of the gradient and columns of W in L2.
-__device__ __forceinline__ void tile_place(int t, int m_tiles, int n_tiles, int& tm, int& tn) {
-    constexpr int kBand = 8;
-    const int band = t / (kBand * n_tiles), in = t - band * (kBand * n_tiles);
-    const int rows = min(kBand, m_tiles - band * kBand);
-    tn = in / rows;
-    tm = band * kBand + in - tn * rows;
 }
 
 template <int FMT, int CG, int NB>

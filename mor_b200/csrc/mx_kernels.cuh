@@ -20,7 +20,9 @@ struct MxMatmulArgs {
     void* out;          // bf16 [m, n]
     int64_t m, n, k;
     int a_fmt, b_fmt;
+    void* workspace;    // mx_matmul_workspace bytes
 };
+size_t mx_matmul_workspace(int64_t m, int64_t n, int64_t k);
 int launch_mx_matmul(const MxMatmulArgs& a, cudaStream_t st);
 
 // mx_grad.cu: out[m, n] = sum_k op(g)[m, k] decode(payload)[k, n]

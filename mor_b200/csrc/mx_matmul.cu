@@ -3,6 +3,8 @@
 // Both operands are K-major with one E8M0 byte for every 32 elements of a row, which is what the instruction multiplies
 // into the product itself: the codes go from global to shared memory by TMA and are never widened.  A tile is 128 rows of
 // one operand (P) by TN rows of the other (Q), 128 bytes of K (256 E2M1 or 128 E4M3 / E5M2 elements) at a time.
+#include <algorithm>
+
 #include "mx_kernels.cuh"
 #include "tcgen05.cuh"
 
@@ -233,6 +235,292 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
     if (warp == 5) { tc_fence_after(); tmem_free<1>(tmem, S::kCols); }
 }
 
+// ---------------------------------------------------------------------------------
+// large products: pairs of CTAs on 256 x 256
+// ---------------------------------------------------------------------------------
+// Scale bytes [rows, groups] in the order the tensor core's copy wants them: for every 128 rows and four groups 512 bytes,
+// 16 for each r mod 32, four for each r / 32, zeros where there is no row or group.  One thread takes 16 groups of a row.
+__global__ void __launch_bounds__(128) tile_scales_kernel(const uint8_t* __restrict__ sa, int64_t rows_a, uint32_t* __restrict__ oa, int blocks_a,
+                                                          const uint8_t* __restrict__ sb, int64_t rows_b, uint32_t* __restrict__ ob, int64_t groups,
+                                                          int kblocks, int fast) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const bool first = (int)blockIdx.x < blocks_a;
+    const int64_t rb = first ? blockIdx.x : blockIdx.x - blocks_a;
+    const uint8_t* s = first ? sa : sb;
+    const int64_t row = rb * 128 + (threadIdx.x & 3) * 32 + (threadIdx.x >> 2);
+    const bool in = row < (first ? rows_a : rows_b);
+    uint32_t* o = (first ? oa : ob) + rb * kblocks * 128 + threadIdx.x;
+    for (int b = blockIdx.y * 4; b < kblocks; b += gridDim.y * 4) {
+        uint32_t w[4] = {};
+        const uint8_t* src = s + row * groups + b * 4;
+        if (in && fast) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));   // groups is a multiple of 16
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        } else if (in) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (b * 4 + i < groups) w[i >> 2] |= (uint32_t)__ldg(src + i) << (8 * (i & 3));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (b + i < kblocks) o[(int64_t)(b + i) * 128] = w[i];
+    }
+}
+
+struct PairArgs {
+    const uint16_t* bias;
+    uint16_t* out;
+    int64_t m, n;
+    uint32_t idesc;
+    int m_tiles, n_tiles, tiles, ksteps, tma_out;
+};
+
+template <bool FP4>
+struct PairShape {
+    static constexpr int kBlk = FP4 ? 2 : 1;
+    static constexpr int kTile = 128 * 128;                                  // bytes of 128 rows of an operand, one step
+    static constexpr int kSfP = kBlk * 512, kSfQ = 2 * kSfP;
+    static constexpr int kSfOff = 2 * kTile, kStage = kSfOff + ((kSfP + kSfQ + 1023) & ~1023);
+    static constexpr int kStages = 5;
+    static constexpr int kOutOff = kStages * kStage, kOutBytes = 128 * 128;  // 128 x 64 results on their way out, one for each half of the columns
+    static constexpr int kSmem = kOutOff + 2 * kOutBytes + 1024;
+    static constexpr int kSfCols = 12 * kBlk;                                // columns of tensor memory for a step's scales
+    static_assert(kSmem <= 227 * 1024 - 2048, "shared memory");
+};
+
+// Warps 0-7 write the results, warp 8 loads, warp 9 issues (in the first CTA) or says that this CTA's operands are there
+// (in the second).  Each CTA loads 128 rows of either operand, A's scales for its rows and B's for all 256 columns.  The
+// accumulator fills half of tensor memory and the scales need some of the rest, so there is one: between two tiles the
+// issuer waits until it is in registers, packed to bf16 (64 of them a thread); the stores go on under the next tile.
+template <bool FP4>
+__global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                                                                const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
+                                                                const __grid_constant__ CUtensorMap map_out, const PairArgs a) {
+    using S = PairShape<FP4>;
+    extern __shared__ uint8_t s_raw[];
+    __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], acc_full, acc_empty, drained;
+    __shared__ uint32_t s_tmem;
+    __shared__ __align__(16) float s_bias[256];
+    uint8_t* smem = s_raw + ((1024 - (smem_u32(s_raw) & 1023)) & 1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank();
+    const int first = (int)(blockIdx.x >> 1), step = (int)(gridDim.x >> 1);
+    if (warp == 8 && lane == 0) {
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(&full[s], rank == 0 ? 2 : 1); mbar_init(&empty[s], 1); }
+        mbar_init(&acc_full, 1);
+        mbar_init(&acc_empty, 16);
+        mbar_init(&drained, 1);
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a));
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b));
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_sa));
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_sb));
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_out));
+    }
+    if (warp == 9) tmem_alloc<2>(&s_tmem, 512);
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    bool ok = true;   // a wait that ran out ends the role; what it would have computed is written as NaN
+    if (warp == 8) {
+        Slot<S::kStages> sl;
+        for (int t = first; t < a.tiles && ok; t += step) {
+            int tm, tn;
+            tile_place(t, a.m_tiles, a.n_tiles, tm, tn);
+            for (int j = 0; j < a.ksteps; ++j) {
+                ok = mbar_wait_warp(&empty[sl.s], sl.phase ^ 1);
+                if (!ok) break;
+                if (elect_one()) {
+                    uint8_t* st = smem + sl.s * S::kStage;
+                    uint64_t* bar = &full[sl.s];
+                    mbar_expect_tx(bar, 2 * S::kTile + S::kSfP + S::kSfQ);
+                    tma_load_2d(st, &map_a, j * 128, tm * 256 + rank * 128, bar);
+                    tma_load_2d(st + S::kTile, &map_b, j * 128, tn * 256 + rank * 128, bar);
+                    tma_load_2d(st + S::kSfOff, &map_sa, j * (S::kBlk * 128), tm * 2 + rank, bar);
+                    tma_load_2d(st + S::kSfOff + S::kSfP, &map_sb, j * (S::kBlk * 128), tn * 2, bar);
+                }
+                __syncwarp();
+                sl.advance();
+            }
+        }
+        if (!ok)   // copies in flight land before the shared memory is handed on: every slot's last round
+            for (int s = 0; s < S::kStages; ++s) mbar_wait_bounded(&full[s], s < sl.s ? sl.phase : sl.phase ^ 1);
+    } else if (warp == 9) {
+        Slot<S::kStages> sl;
+        if (rank == 1) {
+            const uint32_t full0 = map_to_rank(smem_u32(&full[0]), 0);
+            const int64_t total = first < a.tiles ? (int64_t)((a.tiles - 1 - first) / step + 1) * a.ksteps : 0;
+            for (int64_t i = 0; i < total; ++i) {
+                if (!mbar_wait_warp(&full[sl.s], sl.phase)) break;
+                if (elect_one()) mbar_arrive_peer(full0 + 8 * sl.s);
+                __syncwarp();
+                sl.advance();
+            }
+        } else {
+            const uint64_t d0 = umma_desc_kmajor(smem_u32(smem));
+            int it = 0;
+            for (int t = first; t < a.tiles && ok; t += step, ++it) {
+                if (it > 0) ok = mbar_wait_warp(&acc_empty, (it - 1) & 1);
+                if (!ok) break;
+                for (int j = 0; j < a.ksteps; ++j) {
+                    ok = mbar_wait_warp(&full[sl.s], sl.phase);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t sf = smem_u32(smem) + sl.s * S::kStage + S::kSfOff;
+                        const uint32_t tp = tmem + 256 + (j & 1) * S::kSfCols, tq = tp + 4 * S::kBlk;
+#pragma unroll
+                        for (int b = 0; b < S::kBlk; ++b) {   // a block is four groups of K: four columns for A's 128 rows, eight for B's 256
+                            tc_copy_scales<2>(tp + 4 * b, sf + 512 * b);
+                            tc_copy_scales<2>(tq + 8 * b, sf + S::kSfP + 512 * b);
+                            tc_copy_scales<2>(tq + 8 * b + 4, sf + 2 * S::kSfP + 512 * b);
+                        }
+                        const uint64_t da = d0 + sl.s * (S::kStage / 16), db = da + S::kTile / 16;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {   // 32 bytes of K each
+                            const uint32_t blk = FP4 ? k >> 1 : 0, id = FP4 ? (k & 1) * 2 : k;
+                            tc_mma_scaled<2, FP4>(tmem, da + 2 * k, db + 2 * k, idesc_with_scale_id(a.idesc, id), tp + 4 * blk, tq + 8 * blk, (j | k) != 0);
+                        }
+                        tc_commit_pair(&empty[sl.s]);
+                        if (j == a.ksteps - 1) tc_commit_pair(&acc_full);
+                    }
+                    __syncwarp();
+                    sl.advance();
+                }
+            }
+            if (!ok) {   // products in flight end before the tensor memory is handed on
+                if (elect_one()) tc_commit_pair(&drained);
+                __syncwarp();
+                mbar_wait_bounded(&drained, 0);
+            }
+        }
+    } else {
+        const int half = warp >> 2, t128 = threadIdx.x & 127;   // columns 128 half ..., accumulator row
+        const uint32_t acc = tmem + half * 128 + ((uint32_t)(warp & 3) << 21);
+        const uint32_t empty0 = map_to_rank(smem_u32(&acc_empty), 0);
+        uint8_t* os = smem + S::kOutOff + half * S::kOutBytes;
+        int it = 0;
+        for (int t = first; t < a.tiles; t += step, ++it) {
+            int tm, tn;
+            tile_place(t, a.m_tiles, a.n_tiles, tm, tn);
+            const int64_t m0 = (int64_t)tm * 256 + rank * 128, n0 = (int64_t)tn * 256 + half * 128;
+            if (a.bias) {
+                named_barrier(1 + half, 128);   // the tile before is through with these
+                s_bias[half * 128 + t128] = n0 + t128 < a.n ? u2f((uint32_t)__ldg(a.bias + n0 + t128) << 16) : 0.0f;
+                named_barrier(1 + half, 128);
+            }
+            ok = ok && mbar_wait_warp(&acc_full, it & 1);
+            tc_fence_after();
+            uint32_t w[64];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t r[32];
+                tmem_load32(acc + 32 * c, r);
+                tmem_wait_loads();
+                if (a.bias) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 v = *reinterpret_cast<const float4*>(&s_bias[half * 128 + 32 * c + e]);
+                        r[e] = f2u(u2f(r[e]) + v.x);
+                        r[e + 1] = f2u(u2f(r[e + 1]) + v.y);
+                        r[e + 2] = f2u(u2f(r[e + 2]) + v.z);
+                        r[e + 3] = f2u(u2f(r[e + 3]) + v.w);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) w[16 * c + e] = ok ? pack_bf16_rne(u2f(r[2 * e + 1]), u2f(r[2 * e])) : 0x7FFF7FFFu;
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (elect_one()) mbar_arrive_peer(empty0);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {   // 64 columns at a time
+                if (t128 == 0) bulk_wait_reads();
+                named_barrier(1 + half, 128);
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    *reinterpret_cast<uint4*>(os + t128 * 128 + ((q ^ (t128 & 7)) << 4)) =
+                        make_uint4(w[32 * c + 4 * q], w[32 * c + 4 * q + 1], w[32 * c + 4 * q + 2], w[32 * c + 4 * q + 3]);
+                fence_async_shared();
+                named_barrier(1 + half, 128);
+                const int64_t nc = n0 + 64 * c;
+                if (a.tma_out) {
+                    if (t128 == 0) {
+                        if (m0 < a.m && nc < a.n) tma_store_2d(&map_out, os, (int)nc, (int)m0);
+                        bulk_commit();
+                    }
+                } else {   // rows that do not start on 16 bytes: a warp writes one row at a time
+                    for (int r = (warp & 3) * 32; r < (warp & 3) * 32 + 32 && m0 + r < a.m; ++r) {
+                        const uint32_t v = *reinterpret_cast<const uint32_t*>(os + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                        uint16_t* o = a.out + (m0 + r) * a.n + nc + 2 * lane;
+                        if (nc + 2 * lane < a.n) o[0] = (uint16_t)v;
+                        if (nc + 2 * lane + 1 < a.n) o[1] = (uint16_t)(v >> 16);
+                    }
+                }
+            }
+        }
+        if (t128 == 0) bulk_wait_reads();
+    }
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();
+    if (warp == 9) { tc_fence_after(); tmem_free<2>(tmem, 512); }
+}
+
+// columns of scale blocks of a row of tiles, padded to whole steps of either format
+inline int64_t scale_blocks(int64_t k) { return ((k / 32 + 3) / 4 + 1) & ~int64_t(1); }
+
+template <bool FP4>
+int go_pair(const MxMatmulArgs& x, cudaStream_t st) {
+    using S = PairShape<FP4>;
+    auto kern = mx_matmul_pair_kernel<FP4>;
+    static SmemOptIn opt;
+    if (!opt(kern, S::kSmem)) return kErrLaunch;
+    const int64_t kb = scale_blocks(x.k), rb_a = (x.m + 127) / 128, rb_b = (x.n + 127) / 128, groups = x.k / 32;
+    auto* sa = static_cast<uint32_t*>(x.workspace);
+    uint32_t* sb = sa + rb_a * kb * 128;
+    PairArgs a = {};
+    a.bias = static_cast<const uint16_t*>(x.bias);
+    a.out = static_cast<uint16_t*>(x.out);
+    a.m = x.m; a.n = x.n;
+    a.m_tiles = (int)((x.m + 255) / 256); a.n_tiles = (int)((x.n + 255) / 256);
+    if ((int64_t)a.m_tiles * a.n_tiles > (1 << 30) || rb_a + rb_b > 0x7FFFFFFF) return kErrTooLarge;
+    a.tiles = a.m_tiles * a.n_tiles;
+    const int64_t row_bytes = FP4 ? x.k / 2 : x.k;
+    a.ksteps = (int)((row_bytes + 127) / 128);
+    a.idesc = idesc_scaled(256, 256, FP4 ? 1u : (uint32_t)x.a_fmt, FP4 ? 1u : (uint32_t)x.b_fmt);
+    a.tma_out = x.n % 8 == 0 && (reinterpret_cast<uintptr_t>(x.out) & 15) == 0;
+    const int fast = groups % 16 == 0 && ((reinterpret_cast<uintptr_t>(x.a_scales) | reinterpret_cast<uintptr_t>(x.b_scales)) & 15) == 0;
+    CUtensorMap ma, mb, msa, msb, mo;
+    if (!make_swizzled_map(&ma, x.a, x.m, row_bytes, row_bytes, 1, 128) || !make_swizzled_map(&mb, x.b, x.n, row_bytes, row_bytes, 1, 128)) return kErrLaunch;
+    if (!make_word_map(&msa, sa, rb_a, kb * 128, S::kBlk * 128, 1) || !make_word_map(&msb, sb, rb_b, kb * 128, S::kBlk * 128, 2)) return kErrLaunch;
+    if (!a.tma_out) mo = ma;
+    else if (!make_swizzled_map(&mo, x.out, x.m, x.n, x.n * 2, 2, 128)) return kErrLaunch;
+    const dim3 grid((unsigned)(rb_a + rb_b), (unsigned)std::min<int64_t>((kb + 3) / 4, 64));
+    if (launch_pdl(tile_scales_kernel, grid, dim3(128), 0, st, x.a_scales, x.m, sa, (int)rb_a, x.b_scales, x.n, sb, groups, (int)kb, fast) != cudaSuccess)
+        return kErrLaunch;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * std::min(a.tiles, sm_count() / 2)));
+    cfg.blockDim = dim3(320);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {2, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, ma, mb, msa, msb, mo, a) == cudaSuccess ? check_launch() : kErrLaunch;
+}
+
+// Pairs where their tiles fill at least half of the pairs
+inline bool takes_pairs(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) * 2 >= sm_count() / 2; }
+
 template <bool FP4, int TN, bool SWAP>
 int go(const CUtensorMap& mp, const CUtensorMap& mq, const MmArgs& a, int64_t tiles, cudaStream_t st) {
     using S = MmShape<FP4, TN>;
@@ -257,6 +545,8 @@ int go(const CUtensorMap& mp, const CUtensorMap& mq, const MmArgs& a, int64_t ti
 
 template <bool FP4>
 int dispatch(const MxMatmulArgs& x, cudaStream_t st) {
+    if (!bind_context()) return kErrLaunch;
+    if (takes_pairs(x.m, x.n)) return go_pair<FP4>(x, st);
     const bool swap = x.m <= 64;
     const int tn = !swap ? 128 : (x.m <= 16 ? 16 : (x.m <= 32 ? 32 : 64));
     MmArgs a = {};
@@ -280,7 +570,6 @@ int dispatch(const MxMatmulArgs& x, cudaStream_t st) {
     a.splits = 1;
     while (a.splits < 8 && tiles * a.splits * 2 <= sm_count() && a.ktiles >= a.splits * 4) a.splits *= 2;
     CUtensorMap mp, mq;
-    if (!bind_context()) return kErrLaunch;
     if (!make_swizzled_map(&mp, p, a.p_rows, row_bytes, row_bytes, 1, kPRows)) return kErrLaunch;
     if (!make_swizzled_map(&mq, q, a.q_rows, row_bytes, row_bytes, 1, tn)) return kErrLaunch;
     if (!swap) return go<FP4, 128, false>(mp, mq, a, tiles, st);
@@ -290,6 +579,10 @@ int dispatch(const MxMatmulArgs& x, cudaStream_t st) {
 }
 
 }  // namespace
+
+size_t mx_matmul_workspace(int64_t m, int64_t n, int64_t k) {
+    return takes_pairs(m, n) ? (size_t)(((m + 127) / 128 + (n + 127) / 128) * scale_blocks(k) * 512) : 0;
+}
 
 int launch_mx_matmul(const MxMatmulArgs& x, cudaStream_t st) {
     return x.a_fmt == kE2M1 ? dispatch<true>(x, st) : dispatch<false>(x, st);

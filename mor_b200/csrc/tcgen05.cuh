@@ -204,6 +204,26 @@ inline bool bind_context() {
     return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
 }
 
+// a place in a ring of N slots and the parity of the round
+template <int N>
+struct Slot {
+    int s = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void advance(int by = 1) {
+        if ((s += by) >= N) { s -= N; phase ^= 1; }
+    }
+};
+
+// Output tile number -> its place: bands of eight rows of tiles, down a band's columns, so that the CTAs at work at one
+// time share rows of one operand and columns of the other in L2.
+__device__ __forceinline__ void tile_place(int t, int m_tiles, int n_tiles, int& tm, int& tn) {
+    constexpr int kBand = 8;
+    const int band = t / (kBand * n_tiles), in = t - band * (kBand * n_tiles);
+    const int rows = min(kBand, m_tiles - band * kBand);
+    tn = in / rows;
+    tm = band * kBand + in - tn * rows;
+}
+
 // row-major matrix of bytes (or bf16) with a row pitch, boxes of 128 bytes x box_rows under the 128-byte swizzle; what lies outside reads as zero
 inline bool make_swizzled_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch_bytes, int elem_bytes,
                               int box_rows) {
@@ -216,6 +236,18 @@ inline bool make_swizzled_map(CUtensorMap* map, const void* base, int64_t rows, 
     return fn(map, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), gdim,
               gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// row-major matrix of 32-bit words, boxes of box_cols x box_rows without swizzle
+inline bool make_word_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int box_cols, int box_rows) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return false;
+    const cuuint64_t gdim[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t gstride[1] = {(cuuint64_t)cols * 4};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+    const cuuint32_t estride[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace morb

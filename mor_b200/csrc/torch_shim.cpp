@@ -414,8 +414,11 @@ at::Tensor mx_matmul(const at::Tensor& a, const at::Tensor& a_scales, const at::
         bi = bias->contiguous();
     }
     at::Tensor out = torch::empty({m, n}, a.options().dtype(torch::kBFloat16));
+    const size_t wsb = mor_b200_mx_matmul_workspace_bytes(m, n, k);
+    at::Tensor ws;
+    if (wsb) ws = workspace(a, wsb);
     check_status(mor_b200_mx_matmul(ac.data_ptr(), as.data_ptr(), bcod.data_ptr(), bs.data_ptr(), m, n, k, (int)a_format, (int)b_format,
-                                    bi.defined() ? bi.data_ptr() : nullptr, out.data_ptr(), cur_stream()),
+                                    bi.defined() ? bi.data_ptr() : nullptr, out.data_ptr(), wsb ? ws.data_ptr() : nullptr, wsb, cur_stream()),
                  "mx_matmul");
     return out;
 }

@@ -167,12 +167,13 @@ def test_product_depths(m, k, fmt):
 
 
 @pytest.mark.parametrize("m,n,k,fmt", [(1, 4096, 4096, E2M1), (24, 4096, 8192, E4M3), (1111, 1003, 2080, E5M2), (2048, 2048, 2048, E2M1),
-                                       (2500, 1536, 1024, E4M3), (4096, 300, 512, E2M1), (300, 4096, 512, E4M3)])
+                                       (2500, 1536, 1024, E4M3), (2305, 1501, 608, E4M3), (2305, 1501, 608, E2M1), (1300, 2056, 32, E2M1),
+                                       (1300, 2056, 160, E5M2), (4096, 2048, 4128, E2M1), (4096, 300, 512, E2M1), (300, 4096, 512, E4M3)])
 def test_product_sizes(m, n, k, fmt):
     check_product(m, n, k, fmt, fmt, bias=True)
 
 
-@pytest.mark.parametrize("m", [1, 300])
+@pytest.mark.parametrize("m", [1, 300, 5000])
 @pytest.mark.parametrize("fmt", [E2M1, E4M3])
 def test_product_every_scale_has_its_place(m, fmt):
     """one group of one row is non-zero at a time, each under a scale of its own: a scale taken from another row or
@@ -187,7 +188,7 @@ def test_product_every_scale_has_its_place(m, fmt):
     check_product(m, n, k, fmt, fmt, b=(p, s))
 
 
-@pytest.mark.parametrize("m", [3, 300])
+@pytest.mark.parametrize("m", [3, 300, 10000])
 @pytest.mark.parametrize("fmt", [E2M1, E4M3])
 def test_product_nan_scales_and_extremes(m, fmt):
     n, k = 200, 512
@@ -211,7 +212,7 @@ def test_product_empty():
     assert z.shape == (4, 64) and not bool(z.any())
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 256, 4096), (40, 512, 4096), (600, 600, 1024)])
+@pytest.mark.parametrize("m,n,k", [(1, 256, 4096), (40, 512, 4096), (600, 600, 1024), (2400, 2300, 1024)])
 def test_product_repeats_bit_for_bit_on_any_stream(m, n, k):
     a, b, _ = product_case(m, n, k, E4M3, E4M3, 8, False)
     args = [t.cuda() for t in (*a, *b)]
@@ -257,12 +258,14 @@ def test_product_strided_and_offset_operands():
 def test_rows_beyond_the_result_are_left_alone():
     """the C entry writes [m, n] and nothing after it"""
     from mor_b200 import cabi
-    for m, n in ((5, 40), (130, 133), (1, 1), (300, 264)):
+    for m, n in ((5, 40), (130, 133), (1, 1), (300, 264), (2305, 1501), (2304, 1032)):
         a, b, _ = product_case(m, n, 96, E4M3, E4M3, 4, False)
         args = [t.cuda() for t in (*a, *b)]
         out = torch.full((m * n + 4096,), 7.0, dtype=torch.bfloat16, device="cuda")
-        cabi.call("mor_b200_mx_matmul", *(t.data_ptr() for t in args), m, n, 96, 0, 0, None, out.data_ptr(), torch.cuda.current_stream().cuda_stream)
-        assert bool((out[m * n:] == 7.0).all())
+        need = cabi.mx_lib().mor_b200_mx_matmul_workspace_bytes(m, n, 96)
+        ws = torch.full((need + 64,), 5, dtype=torch.uint8, device="cuda")
+        cabi.call("mor_b200_mx_matmul", *(t.data_ptr() for t in args), m, n, 96, 0, 0, None, out.data_ptr(), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+        assert bool((out[m * n:] == 7.0).all()) and bool((ws[need:] == 5).all())
         assert torch.equal(out[:m * n].view(m, n), ops().mx_matmul(*args, m, n, 96, 0, 0))
 
 

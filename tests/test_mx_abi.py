@@ -15,11 +15,11 @@ HEADER = os.path.join(ROOT, "include", "mor_b200_mx.h")
 
 def declared():
     text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
-    return sorted(set(re.findall(r"MOR_B200_MX_API\s+int\s+(mor_b200_mx_\w+)\s*\(", text)))
+    return sorted(set(re.findall(r"MOR_B200_MX_API\s+\w+\s+(mor_b200_mx_\w+)\s*\(", text)))
 
 
 def test_header_library_and_binding_agree():
-    assert len(declared()) == 4
+    assert len(declared()) == 5
     out = subprocess.run(["nm", "-D", "--defined-only", cabi.MX_LIB_PATH], capture_output=True, text=True).stdout
     assert sorted(l.split()[-1] for l in out.splitlines() if " T " in l) == declared()
     assert sorted(cabi.MX_SIGNATURES) == declared()
@@ -75,19 +75,25 @@ def test_argument_errors_come_back_as_status_codes():
     assert d(p, p, p, 0, 1 << 40, 64, 32, 0, None) == -5
     assert d(None, None, None, 0, 0, 64, 32, 0, None) == 0
     m = L.mor_b200_mx_matmul
-    assert m(p, p, p, p, 4, 4, 64, 4, 0, None, p, None) == -1
-    assert m(p, p, p, p, 4, 4, 64, 3, 3, None, p, None) == -1
-    assert m(p, p, p, p, 4, 4, 0, 0, 0, None, p, None) == -1
-    assert m(p, p, p, p, -4, 4, 64, 0, 0, None, p, None) == -1
-    assert m(p, p, p, p, 4, 4, 48, 0, 0, None, p, None) == -2
-    assert m(p + 8, p, p, p, 4, 4, 64, 0, 0, None, p, None) == -2
-    assert m(p, p, p + 8, p, 4, 4, 64, 0, 0, None, p, None) == -2
-    assert m(p, p, p, p, 4, 4, 64, 0, 0, p + 1, p, None) == -2
-    assert m(p, p, p, p, 4, 4, 64, 0, 0, None, p + 1, None) == -2
-    assert m(p, None, p, p, 4, 4, 64, 0, 0, None, p, None) == -1
-    assert m(p, p, p, p, 4, 4, 64, 0, 0, None, None, None) == -1
-    assert m(p, p, p, p, 4, 1 << 40, 64, 0, 0, None, p, None) == -5
-    assert m(None, None, None, None, 0, 4, 64, 0, 0, None, None, None) == 0
+    assert m(p, p, p, p, 4, 4, 64, 4, 0, None, p, None, 0, None) == -1
+    assert m(p, p, p, p, 4, 4, 64, 3, 3, None, p, None, 0, None) == -1
+    assert m(p, p, p, p, 4, 4, 0, 0, 0, None, p, None, 0, None) == -1
+    assert m(p, p, p, p, -4, 4, 64, 0, 0, None, p, None, 0, None) == -1
+    assert m(p, p, p, p, 4, 4, 48, 0, 0, None, p, None, 0, None) == -2
+    assert m(p + 8, p, p, p, 4, 4, 64, 0, 0, None, p, None, 0, None) == -2
+    assert m(p, p, p + 8, p, 4, 4, 64, 0, 0, None, p, None, 0, None) == -2
+    assert m(p, p, p, p, 4, 4, 64, 0, 0, p + 1, p, None, 0, None) == -2
+    assert m(p, p, p, p, 4, 4, 64, 0, 0, None, p + 1, None, 0, None) == -2
+    assert m(p, None, p, p, 4, 4, 64, 0, 0, None, p, None, 0, None) == -1
+    assert m(p, p, p, p, 4, 4, 64, 0, 0, None, None, None, 0, None) == -1
+    assert m(p, p, p, p, 4, 1 << 40, 64, 0, 0, None, p, None, 0, None) == -5
+    assert m(None, None, None, None, 0, 4, 64, 0, 0, None, None, None, 0, None) == 0
+    assert m(p, p, p, p, 4096, 4096, 64, 0, 0, None, p, None, 0, None) == -3      # large products need the workspace
+    assert m(p, p, p, p, 4096, 4096, 64, 0, 0, None, p, p, 4096, None) == -3
+    assert m(p, p, p, p, 4096, 4096, 64, 0, 0, None, p, p + 8, 1 << 20, None) == -3
+    w = L.mor_b200_mx_matmul_workspace_bytes
+    assert w(4096, 4096, 64) == 64 * 2 * 512 and w(4097, 4096, 4096) == 65 * 32 * 512 and w(1, 4096, 4096) == 0
+    assert w(0, 1, 32) == 0 and w(4096, 4096, 48) == 0 and w(1 << 40, 1, 32) == 0
     g = L.mor_b200_mx_matmul_grad
     assert g(p, 64, p, p, 4, 64, 64, 2, 0, p, None) == -1
     assert g(p, 64, p, p, 4, 64, 64, 0, 2, p, None) == -1
