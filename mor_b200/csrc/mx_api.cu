@@ -58,7 +58,8 @@ int mor_b200_mx_matmul(const void* a, const void* a_scales, const void* b, const
     if (m == 0 || n == 0) return kOk;
     if (!a || !a_scales || !b || !b_scales || !out) return kErrInvalidArgument;
     if (too_large(m) || too_large(n) || too_large(k)) return kErrTooLarge;
-    if (!aligned(a, 16) || !aligned(b, 16) || !aligned(out, 2) || !aligned(bias, 2)) return kErrUnsupportedShape;
+    if (!aligned(a, 16) || !aligned(b, 16) || !aligned(a_scales, 4) || !aligned(b_scales, 4) || !aligned(out, 2) || !aligned(bias, 2))
+        return kErrUnsupportedShape;
     const size_t need = mx_matmul_workspace(m, n, k);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return kErrWorkspace;
     const MxMatmulArgs x{a, b, static_cast<const uint8_t*>(a_scales), static_cast<const uint8_t*>(b_scales), bias, out, m, n, k, a_format, b_format, workspace};

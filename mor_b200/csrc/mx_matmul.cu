@@ -20,7 +20,7 @@ struct MmArgs {
     int64_t ldo;              // row pitch of out (= n)
     int64_t p_tiles;
     uint32_t idesc;
-    int ktiles, splits, fast_scales, vec_out;
+    int ktiles, splits, tiled_scales, vec_out;
 };
 
 constexpr int kPRows = 128;
@@ -28,7 +28,7 @@ constexpr int kPRows = 128;
 template <bool FP4, int TN>
 struct MmShape {
     static constexpr int kBlk = FP4 ? 2 : 1;                       // 512-byte scale blocks (128 rows x 4 groups) of P per step
-    static constexpr int kQBlk = kBlk * ((TN + 127) / 128);
+    static constexpr int kQBlk = kBlk;
     static constexpr int kPBytes = kPRows * 128, kQBytes = TN * 128;
     static constexpr int kSfOff = kPBytes + kQBytes;
     static constexpr int kStage = (kSfOff + (kBlk + kQBlk) * 512 + 1023) & ~1023;
@@ -41,31 +41,24 @@ struct MmShape {
 };
 
 // Scale bytes of one row for one step: four a block, to the place the tensor core's copy takes them from (row r of 128:
-// 16 bytes for each r mod 32, four for each r / 32).  Rows and groups outside read as zero, a finite scale.
+// 16 bytes for each r mod 32, four for each r / 32).  Rows and groups outside read as zero, a finite scale.  The bytes of
+// a block lie on four bytes: groups is a multiple of four here.
 template <int BLK>
-__device__ __forceinline__ void load_scales(uint32_t dst, const uint8_t* s, int64_t row, int64_t rows, int64_t groups, int64_t g0, bool fast) {
+__device__ __forceinline__ void load_scales(uint32_t dst, const uint8_t* s, int64_t row, int64_t rows, int64_t groups, int64_t g0) {
 #pragma unroll
     for (int b = 0; b < BLK; ++b) {
         const int64_t g = g0 + 4 * b;
         const bool in = row < rows && g < groups;
-        const uint8_t* src = s + (in ? row * groups + g : 0);
-        if (fast) {
-            cp_async4(dst + b * 512, src, in ? 4 : 0);
-        } else {
-            uint32_t w = 0;
-            if (in) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (g + i < groups) w |= (uint32_t)__ldg(src + i) << (8 * i);
-            }
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + b * 512), "r"(w) : "memory");
-        }
+        cp_async4(dst + b * 512, s + (in ? row * groups + g : 0), in ? 4 : 0);
     }
 }
 
 // SWAP: P is B (rows of out's columns) and Q is A, so that few tokens fill a narrow tile of many weight rows.
+// Warps 0-3 fetch scale bytes (unless a kernel ahead has put them in order, then warp 4 does) and write the result, warp 4
+// loads, warp 5 issues.
 template <bool FP4, int TN, bool SWAP>
 __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                                                           const __grid_constant__ CUtensorMap map_sp, const __grid_constant__ CUtensorMap map_sq,
                                                            const MmArgs a) {
     using S = MmShape<FP4, TN>;
     constexpr int kGroupsPerStep = FP4 ? 8 : 4;
@@ -76,13 +69,13 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     const int split = (int)(blockIdx.x % (unsigned)a.splits);
-    const int64_t tile = blockIdx.x / (unsigned)a.splits;
-    const int64_t p0 = (tile % a.p_tiles) * kPRows, q0 = (tile / a.p_tiles) * TN;
+    const int64_t tile = blockIdx.x / (unsigned)a.splits, tp = tile % a.p_tiles, tq = tile / a.p_tiles;
+    const int64_t p0 = tp * kPRows, q0 = tq * TN;
     const int k_first = (int)((int64_t)a.ktiles * split / a.splits), k_last = (int)((int64_t)a.ktiles * (split + 1) / a.splits);
     const int n = k_last - k_first;
 
     if (warp == 4 && lane == 0) {
-        for (int s = 0; s < S::kStages; ++s) { mbar_init(&full[s], 1 + 128); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(&full[s], a.tiled_scales ? 1 : 1 + 128); mbar_init(&empty[s], 1); }
         mbar_init(&acc_done, 1);
         mbar_init(&drained, 1);
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_p));
@@ -98,67 +91,75 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
 
     bool ok = true;   // a wait that ran out ends the role's loop; the tile is then written as NaN
     if (warp == 4) {
-        if (lane == 0) {
-            int i = 0;
-            for (; i < n && ok; ++i) {
-                const int s = i % S::kStages;
-                if (i >= S::kStages) ok = mbar_wait_bounded(&empty[s], (i / S::kStages - 1) & 1);
-                if (!ok) break;
-                uint8_t* st = smem + s * S::kStage;
-                mbar_expect_tx(&full[s], S::kPBytes + S::kQBytes);
+        Slot<S::kStages> sl;
+        for (int i = 0; i < n; ++i) {
+            ok = mbar_wait_warp(&empty[sl.s], sl.phase ^ 1);
+            if (!ok) break;
+            if (elect_one()) {
+                uint8_t* st = smem + sl.s * S::kStage;
+                uint64_t* bar = &full[sl.s];
                 const int x = (k_first + i) * 128;
-                tma_load_2d(st, &map_p, x, (int)p0, &full[s]);
-                tma_load_2d(st + S::kPBytes, &map_q, x, (int)q0, &full[s]);
+                mbar_expect_tx(bar, S::kPBytes + S::kQBytes + (a.tiled_scales ? (S::kBlk + S::kQBlk) * 512 : 0));
+                tma_load_2d(st, &map_p, x, (int)p0, bar);
+                tma_load_2d(st + S::kPBytes, &map_q, x, (int)q0, bar);
+                if (a.tiled_scales) {
+                    tma_load_2d(st + S::kSfOff, &map_sp, x * S::kBlk, (int)tp, bar);   // 128 words a block
+                    tma_load_2d(st + S::kSfOff + S::kBlk * 512, &map_sq, x * S::kBlk, (int)(q0 / 128), bar);
+                }
             }
-            if (!ok)   // copies in flight land before the shared memory is handed on
-                for (int j = i > S::kStages ? i - S::kStages : 0; j < i; ++j) mbar_wait_bounded(&full[j % S::kStages], (j / S::kStages) & 1);
+            __syncwarp();
+            sl.advance();
         }
-        __syncwarp();
+        if (!ok)   // copies in flight land before the shared memory is handed on: every slot's last round
+            for (int s = 0; s < S::kStages; ++s) mbar_wait_bounded(&full[s], s < sl.s ? sl.phase : sl.phase ^ 1);
     } else if (warp == 5) {
-        if (lane == 0) {
-            for (int i = 0; i < n; ++i) {
-                const int s = i % S::kStages;
-                ok = mbar_wait_bounded(&full[s], (i / S::kStages) & 1);
-                if (!ok) break;
-                fence_async_shared();   // the scale bytes came by ordinary copies, the tensor core reads them through its own path
-                tc_fence_after();
-                const uint32_t st = smem_u32(smem + s * S::kStage);
+        Slot<S::kStages> sl;
+        const uint64_t d0 = umma_desc_kmajor(smem_u32(smem));
+        for (int i = 0; i < n; ++i) {
+            ok = mbar_wait_warp(&full[sl.s], sl.phase);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+                fence_async_shared();   // scale bytes that came by ordinary copies; the tensor core reads through its own path
+                const uint32_t sf = smem_u32(smem) + sl.s * S::kStage + S::kSfOff;
                 const uint32_t sfp = tmem + TN + (i & 1) * S::kSfCols, sfq = sfp + 4 * S::kBlk;
 #pragma unroll
-                for (int b = 0; b < S::kBlk + S::kQBlk; ++b) tc_copy_scales<1>(sfp + 4 * b, st + S::kSfOff + 512 * b);
-                const uint64_t dp = umma_desc_kmajor(st), dq = umma_desc_kmajor(st + S::kPBytes);
+                for (int b = 0; b < S::kBlk + S::kQBlk; ++b) tc_copy_scales<1>(sfp + 4 * b, sf + 512 * b);
+                const uint64_t dp = d0 + sl.s * (S::kStage / 16), dq = dp + S::kPBytes / 16;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {   // 32 bytes of K each
                     const uint32_t blk = FP4 ? k >> 1 : 0, id = FP4 ? (k & 1) * 2 : k;
-                    tc_mma_scaled<1, FP4>(tmem, dp + 2 * k, dq + 2 * k, idesc_with_scale_id(a.idesc, id), sfp + 4 * blk,
-                                          sfq + 4 * blk * ((TN + 127) / 128), (i | k) != 0);
+                    tc_mma_scaled<1, FP4>(tmem, dp + 2 * k, dq + 2 * k, idesc_with_scale_id(a.idesc, id), sfp + 4 * blk, sfq + 4 * blk, (i | k) != 0);
                 }
-                tc_commit(&empty[s]);
+                tc_commit(&empty[sl.s]);
+                if (i == n - 1) tc_commit(&acc_done);
             }
-            tc_commit(ok ? &acc_done : &drained);
-            if (!ok) mbar_wait_bounded(&drained, 0);
+            __syncwarp();
+            sl.advance();
         }
-        __syncwarp();
+        if (!ok) {   // products in flight end before the tensor memory is handed on
+            if (elect_one()) tc_commit(&drained);
+            __syncwarp();
+            mbar_wait_bounded(&drained, 0);
+        }
     } else {
-        const int t = threadIdx.x;   // 0..127
-        const uint32_t place = (t & 31) * 16 + (t >> 5) * 4;
-        for (int i = 0; i < n; ++i) {
-            const int s = i % S::kStages;
-            if (i >= S::kStages) ok = mbar_wait_bounded(&empty[s], (i / S::kStages - 1) & 1);
-            ok = __all_sync(0xFFFFFFFFu, ok);
-            if (!ok) break;
-            const uint32_t sf = smem_u32(smem + s * S::kStage + S::kSfOff) + place;
-            const int64_t g0 = (int64_t)(k_first + i) * kGroupsPerStep;
-            load_scales<S::kBlk>(sf, a.sp, p0 + t, a.p_rows, a.groups, g0, a.fast_scales);
-#pragma unroll
-            for (int h = 0; h < (TN + 127) / 128; ++h)
-                if (h * 128 + t < TN)
-                    load_scales<S::kBlk>(sf + 512 * (S::kBlk + h), a.sq, q0 + h * 128 + t, a.q_rows, a.groups, g0, a.fast_scales);
-            cp_async_arrive(&full[s]);
+        if (!a.tiled_scales) {
+            const int t = threadIdx.x;   // 0..127
+            const uint32_t place = (t & 31) * 16 + (t >> 5) * 4;
+            Slot<S::kStages> sl;
+            for (int i = 0; i < n; ++i) {
+                ok = mbar_wait_warp(&empty[sl.s], sl.phase ^ 1);
+                if (!ok) break;
+                const uint32_t sf = smem_u32(smem + sl.s * S::kStage + S::kSfOff) + place;
+                const int64_t g0 = (int64_t)(k_first + i) * kGroupsPerStep;
+                load_scales<S::kBlk>(sf, a.sp, p0 + t, a.p_rows, a.groups, g0);
+                if (t < TN) load_scales<S::kBlk>(sf + 512 * S::kBlk, a.sq, q0 + t, a.q_rows, a.groups, g0);
+                cp_async_arrive(&full[sl.s]);
+                sl.advance();
+            }
+            cp_async_wait_all();
         }
-        cp_async_wait_all();
-        ok = ok && mbar_wait_bounded(&acc_done, 0);
-        ok = __all_sync(0xFFFFFFFFu, ok);
+        ok = ok && mbar_wait_warp(&acc_done, 0);
         tc_fence_after();
     }
 
@@ -474,35 +475,40 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
 // columns of scale blocks of a row of tiles, padded to whole steps of either format
 inline int64_t scale_blocks(int64_t k) { return ((k / 32 + 3) / 4 + 1) & ~int64_t(1); }
 
+// The scale bytes of both operands in tensor-core order, in the workspace, and the maps that load them: BLK blocks of one
+// row of tiles for A, of b_rows of them for B
+bool tile_scales(const MxMatmulArgs& x, int blk, int b_rows, CUtensorMap* map_a, CUtensorMap* map_b, cudaStream_t st) {
+    const int64_t kb = scale_blocks(x.k), rb_a = (x.m + 127) / 128, rb_b = (x.n + 127) / 128, groups = x.k / 32;
+    auto* sa = static_cast<uint32_t*>(x.workspace);
+    uint32_t* sb = sa + rb_a * kb * 128;
+    if (!make_word_map(map_a, sa, rb_a, kb * 128, blk * 128, 1) || !make_word_map(map_b, sb, rb_b, kb * 128, blk * 128, b_rows)) return false;
+    const int fast = groups % 16 == 0 && ((reinterpret_cast<uintptr_t>(x.a_scales) | reinterpret_cast<uintptr_t>(x.b_scales)) & 15) == 0;
+    const dim3 grid((unsigned)(rb_a + rb_b), (unsigned)std::min<int64_t>((kb + 3) / 4, 64));
+    return launch_pdl(tile_scales_kernel, grid, dim3(128), 0, st, x.a_scales, x.m, sa, (int)rb_a, x.b_scales, x.n, sb, groups, (int)kb, fast) == cudaSuccess;
+}
+
 template <bool FP4>
 int go_pair(const MxMatmulArgs& x, cudaStream_t st) {
     using S = PairShape<FP4>;
     auto kern = mx_matmul_pair_kernel<FP4>;
     static SmemOptIn opt;
     if (!opt(kern, S::kSmem)) return kErrLaunch;
-    const int64_t kb = scale_blocks(x.k), rb_a = (x.m + 127) / 128, rb_b = (x.n + 127) / 128, groups = x.k / 32;
-    auto* sa = static_cast<uint32_t*>(x.workspace);
-    uint32_t* sb = sa + rb_a * kb * 128;
     PairArgs a = {};
     a.bias = static_cast<const uint16_t*>(x.bias);
     a.out = static_cast<uint16_t*>(x.out);
     a.m = x.m; a.n = x.n;
     a.m_tiles = (int)((x.m + 255) / 256); a.n_tiles = (int)((x.n + 255) / 256);
-    if ((int64_t)a.m_tiles * a.n_tiles > (1 << 30) || rb_a + rb_b > 0x7FFFFFFF) return kErrTooLarge;
+    if ((int64_t)a.m_tiles * a.n_tiles > (1 << 30)) return kErrTooLarge;
     a.tiles = a.m_tiles * a.n_tiles;
     const int64_t row_bytes = FP4 ? x.k / 2 : x.k;
     a.ksteps = (int)((row_bytes + 127) / 128);
     a.idesc = idesc_scaled(256, 256, FP4 ? 1u : (uint32_t)x.a_fmt, FP4 ? 1u : (uint32_t)x.b_fmt);
     a.tma_out = x.n % 8 == 0 && (reinterpret_cast<uintptr_t>(x.out) & 15) == 0;
-    const int fast = groups % 16 == 0 && ((reinterpret_cast<uintptr_t>(x.a_scales) | reinterpret_cast<uintptr_t>(x.b_scales)) & 15) == 0;
     CUtensorMap ma, mb, msa, msb, mo;
     if (!make_swizzled_map(&ma, x.a, x.m, row_bytes, row_bytes, 1, 128) || !make_swizzled_map(&mb, x.b, x.n, row_bytes, row_bytes, 1, 128)) return kErrLaunch;
-    if (!make_word_map(&msa, sa, rb_a, kb * 128, S::kBlk * 128, 1) || !make_word_map(&msb, sb, rb_b, kb * 128, S::kBlk * 128, 2)) return kErrLaunch;
     if (!a.tma_out) mo = ma;
     else if (!make_swizzled_map(&mo, x.out, x.m, x.n, x.n * 2, 2, 128)) return kErrLaunch;
-    const dim3 grid((unsigned)(rb_a + rb_b), (unsigned)std::min<int64_t>((kb + 3) / 4, 64));
-    if (launch_pdl(tile_scales_kernel, grid, dim3(128), 0, st, x.a_scales, x.m, sa, (int)rb_a, x.b_scales, x.n, sb, groups, (int)kb, fast) != cudaSuccess)
-        return kErrLaunch;
+    if (!tile_scales(x, S::kBlk, 2, &msa, &msb, st)) return kErrLaunch;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(2 * std::min(a.tiles, sm_count() / 2)));
     cfg.blockDim = dim3(320);
@@ -518,11 +524,15 @@ int go_pair(const MxMatmulArgs& x, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, kern, ma, mb, msa, msb, mo, a) == cudaSuccess ? check_launch() : kErrLaunch;
 }
 
+// Few tokens read the weights' scales once and in passing; more of them, and rows of scales that do not lie on four bytes,
+// are worth the kernel that puts the scales in order
+inline bool tiles_scales(int64_t m, int64_t k) { return m > 64 || k % 128 != 0; }
+
 // Pairs where their tiles fill at least half of the pairs
-inline bool takes_pairs(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) * 2 >= sm_count() / 2; }
+inline bool takes_pairs(int64_t m, int64_t n) { return m > 64 && ((m + 255) / 256) * ((n + 255) / 256) * 2 >= sm_count() / 2; }
 
 template <bool FP4, int TN, bool SWAP>
-int go(const CUtensorMap& mp, const CUtensorMap& mq, const MmArgs& a, int64_t tiles, cudaStream_t st) {
+int go(const CUtensorMap& mp, const CUtensorMap& mq, const CUtensorMap& msp, const CUtensorMap& msq, const MmArgs& a, int64_t tiles, cudaStream_t st) {
     using S = MmShape<FP4, TN>;
     auto k = mx_matmul_kernel<FP4, TN, SWAP>;
     static SmemOptIn opt;
@@ -540,7 +550,7 @@ int go(const CUtensorMap& mp, const CUtensorMap& mq, const MmArgs& a, int64_t ti
     attr[1].val.clusterDim = {(unsigned)a.splits, 1, 1};
     cfg.attrs = attr;
     cfg.numAttrs = a.splits > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, k, mp, mq, a) == cudaSuccess ? check_launch() : kErrLaunch;
+    return cudaLaunchKernelEx(&cfg, k, mp, mq, msp, msq, a) == cudaSuccess ? check_launch() : kErrLaunch;
 }
 
 template <bool FP4>
@@ -564,24 +574,27 @@ int dispatch(const MxMatmulArgs& x, cudaStream_t st) {
     a.ktiles = (int)((row_bytes + 127) / 128);
     const int pf = swap ? x.b_fmt : x.a_fmt, qf = swap ? x.a_fmt : x.b_fmt;
     a.idesc = idesc_scaled(128, tn, FP4 ? 1u : (uint32_t)pf, FP4 ? 1u : (uint32_t)qf);
-    a.fast_scales = a.groups % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.sp) | reinterpret_cast<uintptr_t>(a.sq)) & 3) == 0;
+    a.tiled_scales = tiles_scales(x.m, x.k);
     a.vec_out = x.n % 8 == 0 && (reinterpret_cast<uintptr_t>(x.out) & 15) == 0;
     const int64_t tiles = a.p_tiles * ((a.q_rows + tn - 1) / tn);
     a.splits = 1;
     while (a.splits < 8 && tiles * a.splits * 2 <= sm_count() && a.ktiles >= a.splits * 4) a.splits *= 2;
-    CUtensorMap mp, mq;
+    CUtensorMap mp, mq, msa, msb;
     if (!make_swizzled_map(&mp, p, a.p_rows, row_bytes, row_bytes, 1, kPRows)) return kErrLaunch;
     if (!make_swizzled_map(&mq, q, a.q_rows, row_bytes, row_bytes, 1, tn)) return kErrLaunch;
-    if (!swap) return go<FP4, 128, false>(mp, mq, a, tiles, st);
-    if (tn == 16) return go<FP4, 16, true>(mp, mq, a, tiles, st);
-    if (tn == 32) return go<FP4, 32, true>(mp, mq, a, tiles, st);
-    return go<FP4, 64, true>(mp, mq, a, tiles, st);
+    if (!a.tiled_scales) msa = msb = mp;   // not used
+    else if (!tile_scales(x, FP4 ? 2 : 1, 1, &msa, &msb, st)) return kErrLaunch;
+    const CUtensorMap &msp = swap ? msb : msa, &msq = swap ? msa : msb;
+    if (!swap) return go<FP4, 128, false>(mp, mq, msp, msq, a, tiles, st);
+    if (tn == 16) return go<FP4, 16, true>(mp, mq, msp, msq, a, tiles, st);
+    if (tn == 32) return go<FP4, 32, true>(mp, mq, msp, msq, a, tiles, st);
+    return go<FP4, 64, true>(mp, mq, msp, msq, a, tiles, st);
 }
 
 }  // namespace
 
 size_t mx_matmul_workspace(int64_t m, int64_t n, int64_t k) {
-    return takes_pairs(m, n) ? (size_t)(((m + 127) / 128 + (n + 127) / 128) * scale_blocks(k) * 512) : 0;
+    return tiles_scales(m, k) ? (size_t)(((m + 127) / 128 + (n + 127) / 128) * scale_blocks(k) * 512) : 0;
 }
 
 int launch_mx_matmul(const MxMatmulArgs& x, cudaStream_t st) {
