@@ -149,6 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
     // A wait that ran out ends the role; what it would have computed is written as NaN.  A slot's first use finds its
     // `empty` barrier in the phase before the first: waiting for the parity opposite to the round's passes at once.
     bool ok = true;
+    const ClusterSum<S::kTN> sums{smem_u32(smem), a.splits, split};
     if (warp == 4) {
         Slot<S::kSA> sa;
         for (int t = first; t < a.tiles && ok; t += step) {
@@ -314,6 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
         static_assert(kRowsPerPass % 8 == 0 && kConvGroups <= S::kSA && kConvGroups <= S::kSB && kConvGroups <= S::kSC, "swizzle, first slots");
     } else {
         int it = 0;
+        const uint32_t sums_to = sums.place(threadIdx.x);
         const uint32_t empty0 = CG == 2 ? map_to_rank(smem_u32(&acc_empty[0]), 0) : smem_u32(&acc_empty[0]);
         int ob = 0;
         for (int t = first; t < a.tiles; t += step, ++it) {
@@ -324,6 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
             ok = ok && mbar_wait_warp(&acc_full[b], (it / 2) & 1);
             tc_fence_after();
             const uint32_t acc = tmem + b * S::kTN + ((uint32_t)warp << 21);
+            if (CG == 1 && a.splits > 1) cluster_sync();   // no CTA is still reading operands; the other warps meet this below
 #pragma unroll 1
             for (int c0 = 0; c0 < S::kTN; c0 += 64) {
                 uint32_t r[2][32];
@@ -334,10 +337,12 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
 #pragma unroll
                     for (int c = 0; c < 32; ++c) r[0][c] = r[1][c] = 0x7FFFFFFFu;
                 }
-                if (a.splits > 1) {
-                    float* part = reinterpret_cast<float*>(smem);   // [column][128 rows]; the operands are no longer needed
+                if (CG == 1 && a.splits > 1) {
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) part[(c0 + c) * 128 + threadIdx.x] = u2f(r[c >> 5][c & 31]);
+                    for (int c = 0; c < 64; c += 4) {
+                        const uint32_t* q = &r[c >> 5][c & 31];
+                        ClusterSum<S::kTN>::push(sums_to + 4 * (c0 + c), q[0], q[1], q[2], q[3]);
+                    }
                 } else {
                     uint8_t* os = smem + S::kOutOff + ob * S::kOutBytes;
                     if (threadIdx.x == 0) bulk_wait_reads_but<1>();   // the store from this buffer before last has read it
@@ -365,30 +370,24 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
         if (threadIdx.x == 0) bulk_wait_reads();
     }
 
-    if (CG == 1 && a.splits > 1) {   // partial sums of one tile in the CTAs of a cluster: each adds up some of the columns, in rank order
+    if (CG == 1 && a.splits > 1) {   // one tile to a CTA: its partial sums meet those of the cluster's other CTAs
         __syncwarp();
+        if (warp >= 4) cluster_sync();
         cluster_sync();
         if (warp < 4) {
+            static_assert(ClusterSum<S::kTN>::kBytes <= S::kOutOff, "partial sums");
             int tm, tn;
             tile_place(first, a.m_tiles, a.n_tiles, tm, tn);
-            const int64_t m = (int64_t)tm * 128 + threadIdx.x, n0 = (int64_t)tn * S::kTN;
-            const uint32_t mine = smem_u32(smem) + 4 * threadIdx.x;
-            for (int c = 8 * split; c < S::kTN && n0 + c < a.n; c += 8 * a.splits) {
-                float sum[8] = {};
-                for (int z = 0; z < a.splits; ++z)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float v;
-                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(mine + (c + e) * 512, z)) : "memory");
-                        sum[e] += v;
-                    }
-                if (m < a.m)
-                    *reinterpret_cast<uint4*>(a.out + m * a.n + n0 + c) = make_uint4(pack_bf16_rne(sum[1], sum[0]), pack_bf16_rne(sum[3], sum[2]),
-                                                                                      pack_bf16_rne(sum[5], sum[4]), pack_bf16_rne(sum[7], sum[6]));
+            constexpr int kLanes = S::kTN / 4;   // a lane takes four columns
+            const int c = (threadIdx.x % kLanes) * 4;
+            const int64_t m0 = (int64_t)tm * 128 + split * sums.rows(), n = (int64_t)tn * S::kTN + c;
+#pragma unroll 4
+            for (int r = threadIdx.x / kLanes; r < sums.rows(); r += 128 / kLanes) {
+                if (m0 + r >= a.m || n >= a.n) break;
+                const float4 v = sums.sum4(r, c);
+                *reinterpret_cast<uint2*>(a.out + (m0 + r) * a.n + n) = make_uint2(pack_bf16_rne(v.y, v.x), pack_bf16_rne(v.w, v.z));
             }
         }
-        __syncwarp();
-        cluster_sync();
     }
     __syncwarp();
     tc_fence_before();

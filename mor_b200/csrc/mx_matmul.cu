@@ -163,74 +163,76 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
         tc_fence_after();
     }
 
+    // The result leaves through shared memory (the operands are no longer needed), where the partial sums of a cluster
+    // meet and neighbouring lanes get neighbouring elements of a row of out.
+    __syncwarp();
+    if (a.splits > 1) cluster_sync();   // no CTA is still reading operands
+    const ClusterSum<TN> sums{smem_u32(smem), a.splits, split};
+    static_assert(ClusterSum<TN>::kBytes <= S::kStages * S::kStage, "partial sums");
     if (warp < 4) {
         const uint32_t lanes = tmem + ((uint32_t)warp << 21);   // lane field of the address: 32 per warp
-        const float bad = u2f(0x7FFFFFFFu);
         constexpr int C = TN < 32 ? 16 : 32;
-        const int64_t p = p0 + threadIdx.x;
+        const uint32_t to = sums.place(threadIdx.x);
 #pragma unroll 1
-        for (int c0 = 0; c0 < TN; c0 += C) {
+        for (int c0 = 0; c0 < TN && q0 + c0 < a.q_rows; c0 += C) {
             uint32_t r[C];
             if constexpr (C == 32) tmem_load32(lanes + c0, r); else tmem_load16(lanes + c0, r);
             tmem_wait_loads();
             if (!ok) {
 #pragma unroll
-                for (int c = 0; c < C; ++c) r[c] = f2u(bad);
+                for (int c = 0; c < C; ++c) r[c] = 0x7FFFFFFFu;
             }
-            if (a.splits > 1) {
-                float* part = reinterpret_cast<float*>(smem);   // [column][128 rows]; the operands are no longer needed
 #pragma unroll
-                for (int c = 0; c < C; ++c) part[(c0 + c) * kPRows + threadIdx.x] = u2f(r[c]);
-            } else if (p < a.p_rows) {
-                if constexpr (SWAP) {
-                    const float b = a.bias ? u2f((uint32_t)__ldg(a.bias + p) << 16) : 0.0f;
+            for (int c = 0; c < C; c += 4)
+                if (q0 + c0 + c < a.q_rows) sums.push(to + 4 * (c0 + c), r[c], r[c + 1], r[c + 2], r[c + 3]);
+        }
+    }
+    __syncwarp();
+    if (a.splits > 1) cluster_sync();
+    else if (warp < 4) named_barrier(1, 128);
+    if (warp < 4) {
+        const int rows = sums.rows(), first_row = split * rows;
+        if constexpr (SWAP) {
+            // out's rows run along P: a lane takes one P row, a warp four tokens at a time
+            for (int i = threadIdx.x; i < rows * (TN / 4); i += 128) {
+                const int r = i % rows, c = i / rows * 4;
+                const int64_t p = p0 + first_row + r;
+                if (p >= a.p_rows || q0 + c >= a.q_rows) continue;
+                const float4 v = sums.sum4(r, c);
+                const float bias = a.bias ? u2f((uint32_t)__ldg(a.bias + p) << 16) : 0.0f;
+                const float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                    for (int c = 0; c < C; ++c)
-                        if (q0 + c0 + c < a.q_rows) a.out[(q0 + c0 + c) * a.ldo + p] = (uint16_t)pack_bf16_rne(0.0f, u2f(r[c]) + b);
+                for (int j = 0; j < 4; ++j)
+                    if (q0 + c + j < a.q_rows) a.out[(q0 + c + j) * a.ldo + p] = (uint16_t)pack_bf16_rne(0.0f, e[j] + bias);
+            }
+        } else {
+            constexpr int kLanes = TN / 4;   // a lane takes four columns
+            const int c = (threadIdx.x % kLanes) * 4;
+            const int64_t q = q0 + c;
+            float bias[4] = {};
+            if (a.bias)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (q + j < a.q_rows) bias[j] = u2f((uint32_t)__ldg(a.bias + q + j) << 16);
+#pragma unroll 4
+            for (int r = threadIdx.x / kLanes; r < rows; r += 128 / kLanes) {
+                const int64_t p = p0 + first_row + r;
+                if (p >= a.p_rows) break;
+                const float4 v = sums.sum4(r, c);
+                uint16_t* o = a.out + p * a.ldo + q;
+                const uint2 w = make_uint2(pack_bf16_rne(v.y + bias[1], v.x + bias[0]), pack_bf16_rne(v.w + bias[3], v.z + bias[2]));
+                if (a.vec_out && q + 4 <= a.q_rows) {
+                    *reinterpret_cast<uint2*>(o) = w;
                 } else {
-                    const int64_t q = q0 + c0;
-                    uint16_t* o = a.out + p * a.ldo + q;
-                    if (a.bias) {
-#pragma unroll
-                        for (int c = 0; c < C; ++c)
-                            if (q + c < a.q_rows) r[c] = f2u(u2f(r[c]) + u2f((uint32_t)__ldg(a.bias + q + c) << 16));
-                    }
-                    if (a.vec_out && q + C <= a.q_rows) {
-#pragma unroll
-                        for (int c = 0; c < C; c += 8)
-                            *reinterpret_cast<uint4*>(o + c) = make_uint4(
-                                pack_bf16_rne(u2f(r[c + 1]), u2f(r[c])), pack_bf16_rne(u2f(r[c + 3]), u2f(r[c + 2])),
-                                pack_bf16_rne(u2f(r[c + 5]), u2f(r[c + 4])), pack_bf16_rne(u2f(r[c + 7]), u2f(r[c + 6])));
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < C; ++c)
-                            if (q + c < a.q_rows) o[c] = (uint16_t)pack_bf16_rne(0.0f, u2f(r[c]));
-                    }
+                    if (q < a.q_rows) o[0] = (uint16_t)w.x;
+                    if (q + 1 < a.q_rows) o[1] = (uint16_t)(w.x >> 16);
+                    if (q + 2 < a.q_rows) o[2] = (uint16_t)w.y;
+                    if (q + 3 < a.q_rows) o[3] = (uint16_t)(w.y >> 16);
                 }
             }
         }
     }
-    if (a.splits > 1) {   // the CTAs of a cluster hold partial sums of one tile: each adds up some of the columns, in rank order
-        cluster_sync();
-        if (warp < 4) {
-            const int64_t p = p0 + threadIdx.x;
-            const uint32_t mine = smem_u32(smem) + 4 * threadIdx.x;
-            for (int c = split; c < TN && q0 + c < a.q_rows; c += a.splits) {
-                float sum = 0.0f;
-                for (int z = 0; z < a.splits; ++z) {
-                    float v;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(mine + c * (kPRows * 4), z)) : "memory");
-                    sum += v;
-                }
-                if (p < a.p_rows) {
-                    const int64_t col = SWAP ? p : q0 + c, row = SWAP ? q0 + c : p;
-                    if (a.bias) sum += u2f((uint32_t)__ldg(a.bias + col) << 16);
-                    a.out[row * a.ldo + col] = (uint16_t)pack_bf16_rne(0.0f, sum);
-                }
-            }
-        }
-        cluster_sync();
-    }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     if (warp == 5) { tc_fence_after(); tmem_free<1>(tmem, S::kCols); }
@@ -575,7 +577,7 @@ int dispatch(const MxMatmulArgs& x, cudaStream_t st) {
     const int pf = swap ? x.b_fmt : x.a_fmt, qf = swap ? x.a_fmt : x.b_fmt;
     a.idesc = idesc_scaled(128, tn, FP4 ? 1u : (uint32_t)pf, FP4 ? 1u : (uint32_t)qf);
     a.tiled_scales = tiles_scales(x.m, x.k);
-    a.vec_out = x.n % 8 == 0 && (reinterpret_cast<uintptr_t>(x.out) & 15) == 0;
+    a.vec_out = x.n % 4 == 0 && (reinterpret_cast<uintptr_t>(x.out) & 7) == 0;   // eight bytes hold four columns
     const int64_t tiles = a.p_tiles * ((a.q_rows + tn - 1) / tn);
     a.splits = 1;
     while (a.splits < 8 && tiles * a.splits * 2 <= sm_count() && a.ktiles >= a.splits * 4) a.splits *= 2;

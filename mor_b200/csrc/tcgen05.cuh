@@ -175,6 +175,35 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity) {
     return __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar, parity)) != 0;
 }
 
+// Sums over the CTAs of a cluster that each hold partial sums of one tile of 128 rows: the CTA of rank z adds up rows
+// [z, z + 1) 128 / splits.  Every CTA pushes its rows to their owners in 16-byte stores (remote loads would wait some 200
+// cycles each) once all are done with the shared memory they land in, then each owner adds in rank order, so results do
+// not depend on timing.  N columns, rows of N + 4 words: neighbouring rows start four banks apart.
+template <int N>
+struct ClusterSum {
+    static constexpr int kPitch = N + 4, kBytes = 128 * kPitch * 4;
+    uint32_t base;      // the same place in every CTA
+    int splits, rank;
+    __device__ __forceinline__ int rows() const { return 128 / splits; }
+    __device__ __forceinline__ uint32_t place(int row) const {   // where this CTA's part of a row goes
+        const int owner = row / rows();
+        return map_to_rank(base, owner) + (uint32_t)((rank * rows() + row - owner * rows()) * kPitch) * 4;
+    }
+    __device__ __forceinline__ static void push(uint32_t to, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+    }
+    __device__ __forceinline__ float4 sum4(int local_row, int col) const {   // after the cluster has met again
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int z = 0; z < splits; ++z) {
+            float4 v;
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                         : "r"(base + (uint32_t)((z * rows() + local_row) * kPitch + col) * 4) : "memory");
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+        return s;
+    }
+};
+
 // four-byte asynchronous copies, zero-filled where `valid` is 0
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int valid) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
