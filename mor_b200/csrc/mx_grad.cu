@@ -429,7 +429,7 @@ int go(const MxGradArgs& x, cudaStream_t st) {
     if constexpr (CG == 2) {
         grid = 2 * std::min(a.tiles, sm_count() / 2);
     } else {
-        while (a.splits < 8 && a.tiles * a.splits * 2 <= sm_count() && a.ksteps >= a.splits * 4) a.splits *= 2;
+        a.splits = k_splits(a.tiles, a.ksteps, sm_count());
         grid = a.splits > 1 ? a.tiles * a.splits : std::min(a.tiles, sm_count());
     }
     CUtensorMap mg, mc, mo;
@@ -451,13 +451,9 @@ int go(const MxGradArgs& x, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, kern, mg, mc, mo, a) == cudaSuccess ? check_launch() : kErrLaunch;
 }
 
-// Pairs where the 256 x 256 tiles fill at least half of the pairs' slots in the last round; single CTAs on 128 x 128, with the sum over
-// k split within a cluster where even those are few, otherwise.
 template <int FMT>
 int pick(const MxGradArgs& x, cudaStream_t st) {
-    const int64_t big = ((x.m + 255) / 256) * ((x.n + 255) / 256);
-    if (big * 2 >= sm_count() / 2) return go<FMT, 2, 128>(x, st);
-    return go<FMT, 1, 128>(x, st);
+    return takes_pairs(x.m, x.n, (x.k + kTK - 1) / kTK, sm_count()) ? go<FMT, 2, 128>(x, st) : go<FMT, 1, 128>(x, st);
 }
 
 }  // namespace

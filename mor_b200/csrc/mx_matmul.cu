@@ -530,9 +530,6 @@ int go_pair(const MxMatmulArgs& x, cudaStream_t st) {
 // are worth the kernel that puts the scales in order
 inline bool tiles_scales(int64_t m, int64_t k) { return m > 64 || k % 128 != 0; }
 
-// Pairs where their tiles fill at least half of the pairs
-inline bool takes_pairs(int64_t m, int64_t n) { return m > 64 && ((m + 255) / 256) * ((n + 255) / 256) * 2 >= sm_count() / 2; }
-
 template <bool FP4, int TN, bool SWAP>
 int go(const CUtensorMap& mp, const CUtensorMap& mq, const CUtensorMap& msp, const CUtensorMap& msq, const MmArgs& a, int64_t tiles, cudaStream_t st) {
     using S = MmShape<FP4, TN>;
@@ -558,8 +555,9 @@ int go(const CUtensorMap& mp, const CUtensorMap& mq, const CUtensorMap& msp, con
 template <bool FP4>
 int dispatch(const MxMatmulArgs& x, cudaStream_t st) {
     if (!bind_context()) return kErrLaunch;
-    if (takes_pairs(x.m, x.n)) return go_pair<FP4>(x, st);
+    const int64_t row_bytes = FP4 ? x.k / 2 : x.k;
     const bool swap = x.m <= 64;
+    if (!swap && takes_pairs(x.m, x.n, (row_bytes + 127) / 128, sm_count())) return go_pair<FP4>(x, st);
     const int tn = !swap ? 128 : (x.m <= 16 ? 16 : (x.m <= 32 ? 32 : 64));
     MmArgs a = {};
     const void *p = swap ? x.b : x.a, *q = swap ? x.a : x.b;
@@ -572,15 +570,13 @@ int dispatch(const MxMatmulArgs& x, cudaStream_t st) {
     a.groups = x.k / 32;
     a.ldo = x.n;
     a.p_tiles = (a.p_rows + kPRows - 1) / kPRows;
-    const int64_t row_bytes = FP4 ? x.k / 2 : x.k;
     a.ktiles = (int)((row_bytes + 127) / 128);
     const int pf = swap ? x.b_fmt : x.a_fmt, qf = swap ? x.a_fmt : x.b_fmt;
     a.idesc = idesc_scaled(128, tn, FP4 ? 1u : (uint32_t)pf, FP4 ? 1u : (uint32_t)qf);
     a.tiled_scales = tiles_scales(x.m, x.k);
     a.vec_out = x.n % 4 == 0 && (reinterpret_cast<uintptr_t>(x.out) & 7) == 0;   // eight bytes hold four columns
     const int64_t tiles = a.p_tiles * ((a.q_rows + tn - 1) / tn);
-    a.splits = 1;
-    while (a.splits < 8 && tiles * a.splits * 2 <= sm_count() && a.ktiles >= a.splits * 4) a.splits *= 2;
+    a.splits = k_splits(tiles, a.ktiles, sm_count());
     CUtensorMap mp, mq, msa, msb;
     if (!make_swizzled_map(&mp, p, a.p_rows, row_bytes, row_bytes, 1, kPRows)) return kErrLaunch;
     if (!make_swizzled_map(&mq, q, a.q_rows, row_bytes, row_bytes, 1, tn)) return kErrLaunch;

@@ -253,6 +253,22 @@ __device__ __forceinline__ void tile_place(int t, int m_tiles, int n_tiles, int&
     tm = band * kBand + in - tn * rows;
 }
 
+// How many CTAs of a cluster share the sum over k of a tile, when single CTAs take tiles of 128 x (n per tile): as many as leave each
+// an SM of its own and four steps.
+inline int k_splits(int64_t tiles, int64_t steps, int sms) {
+    int s = 1;
+    while (s < 8 && tiles * s * 2 <= sms && steps >= s * 4) s *= 2;
+    return s;
+}
+// Pairs of CTAs on 256 x 256 or single ones on 128 x 128?  A pair takes a step in about the time of a single CTA with four
+// times the result, so pairs win unless few tiles let single CTAs split the sum: each step saved is worth about 0.3 us,
+// meeting in the cluster costs about 4.  Measured on both sides: 128 x 4096 x 4096 E4M3 (32 steps, four splits) 15.5 us in pairs, 12.6 single;
+// 4-bit (16 steps) 11.0 and 11.3; 512 x 1024 x 8192 E4M3 24.1 and 15.0; 1024^3 8.3 and 9.9; 1536 x 1536 x 4096 16.3 and 20.6.
+inline bool takes_pairs(int64_t m, int64_t n, int64_t steps, int sms) {
+    const int s = k_splits(((m + 127) / 128) * ((n + 127) / 128), steps, sms);
+    return steps - steps / s < 14;
+}
+
 // row-major matrix of bytes (or bf16) with a row pitch, boxes of 128 bytes x box_rows under the 128-byte swizzle; what lies outside reads as zero
 inline bool make_swizzled_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch_bytes, int elem_bytes,
                               int box_rows) {
