@@ -56,40 +56,47 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
 // pattern's: moved there, the pattern stands for the value times 2^-120 (E4M3; 2^-112, 2^-126 for the others), subnormal
 // codes included, since both formats count subnormals alike.  One multiplication by 2^(scale - 127 + 120) undoes that and
 // applies the scale, with the only rounding there is.  It serves every scale whose product with 2^120 a bf16 holds and
-// every code that is a number; `odd` is set for the rest, which widen8_any takes.
+// every code that is a number; `odd` gets a bit of kOdd for the rest, which widen8_any takes.  A byte permutation that repeats
+// each code's sign up to the top of its half word leaves one shift and one mask for two codes: the widening warps fill
+// the integer pipe, so each instruction here shows in the kernel's time.
+constexpr uint32_t kOdd = 0x80808180u;
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t permute(uint32_t a, uint32_t b) {   // with the sign-repeating selectors 8-15, which __byte_perm drops
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "n"(SEL));
+    return r;
+}
 template <int FMT>
 __device__ __forceinline__ uint4 widen8(uint2 c, uint32_t scale, uint32_t& odd) {
     constexpr uint32_t lift = FMT == kE4M3 ? 120u : (FMT == kE5M2 ? 112u : 126u);
     uint32_t o[4];
     if constexpr (FMT == kE2M1) {
+        const uint32_t lo = (c.x << 4) & 0xF0F0F0F0u, hi = c.x & 0xF0F0F0F0u;   // even and odd columns' codes on top of their bytes
+        o[0] = (permute<0xC480u>(lo, hi) << 2) & 0x81C081C0u;
+        o[1] = (permute<0xD591u>(lo, hi) << 2) & 0x81C081C0u;
+        o[2] = (permute<0xE6A2u>(lo, hi) << 2) & 0x81C081C0u;
+        o[3] = (permute<0xF7B3u>(lo, hi) << 2) & 0x81C081C0u;
+    } else if constexpr (FMT == kE2M3) {
+        const uint32_t w[2] = {c.x << 2, c.y << 2};                             // six bits: sign to the top of the byte
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {   // nibbles 2i, 2i + 1 to the low ends of two halves
-            const uint32_t p = __byte_perm(c.x >> (8 * i), (c.x >> (8 * i)) >> 4, 0x0400) & 0x000F000Fu;
-            o[i] = ((p << 12) & 0x80008000u) | ((p << 6) & 0x01C001C0u);
+        for (int i = 0; i < 2; ++i) {
+            o[2 * i] = (permute<0x9180u>(w[i], 0) << 2) & 0x81F081F0u;
+            o[2 * i + 1] = (permute<0xB3A2u>(w[i], 0) << 2) & 0x81F081F0u;
         }
     } else {
+        constexpr int sh = FMT == kE4M3 ? 4 : 5;
+        constexpr uint32_t mask = FMT == kE4M3 ? 0x87F087F0u : 0x8FE08FE0u;
         const uint32_t w[2] = {c.x, c.y};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            if constexpr (FMT == kE2M3) {
-                const uint32_t lo = __byte_perm(w[i], 0, 0x4140), hi = __byte_perm(w[i], 0, 0x4342);
-                o[2 * i] = ((lo << 10) & 0x80008000u) | ((lo << 4) & 0x01F001F0u);
-                o[2 * i + 1] = ((hi << 10) & 0x80008000u) | ((hi << 4) & 0x01F001F0u);
-            } else {
-                constexpr int sh = FMT == kE4M3 ? 4 : 3;
-                constexpr uint32_t mask = FMT == kE4M3 ? 0x07F007F0u : 0x0FE00FE0u;
-                const uint32_t lo = __byte_perm(w[i], 0, 0x1404), hi = __byte_perm(w[i], 0, 0x3424);
-                o[2 * i] = (lo & 0x80008000u) | ((lo >> sh) & mask);
-                o[2 * i + 1] = (hi & 0x80008000u) | ((hi >> sh) & mask);
-            }
+            o[2 * i] = (permute<0x9180u>(w[i], 0) << sh) & mask;
+            o[2 * i + 1] = (permute<0xB3A2u>(w[i], 0) << sh) & mask;
         }
+        constexpr uint32_t past = FMT == kE4M3 ? 0x01010101u : 0x04040404u;     // carries into bit 7 from 0x7F, from 0x7C up
+        odd |= (((c.x & 0x7F7F7F7Fu) + past) | ((c.y & 0x7F7F7F7Fu) + past)) & 0x80808080u;
     }
-    const uint32_t up = ((scale + lift) & 0xFFu) * 0x00800080u;
-    odd |= scale + lift > 254u ? 0x80u : 0u;
-    if constexpr (FMT == kE4M3 || FMT == kE5M2) {
-        constexpr uint32_t past = FMT == kE4M3 ? 0x01010101u : 0x04040404u;   // carries into bit 7 from 0x7F, from 0x7C up
-        odd |= ((c.x & 0x7F7F7F7Fu) + past) | ((c.y & 0x7F7F7F7Fu) + past);
-    }
+    const uint32_t up = scale * 0x00800080u + lift * 0x00800080u;               // both halves; right while scale + lift < 255
+    odd |= (scale + lift + 1u) & 0x100u;
     return make_uint4(mul_bf16x2(o[0], up), mul_bf16x2(o[1], up), mul_bf16x2(o[2], up), mul_bf16x2(o[3], up));
 }
 template <int FMT>
@@ -299,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
 #pragma unroll
             for (int p = 0; p < kPasses; ++p)   // passes are a multiple of eight rows apart: the same swizzle
                 *reinterpret_cast<uint4*>(bs + p * (kRowsPerPass * 128)) = widen8<FMT>(c[p], k8[p], odd);
-            if (odd & 0x80808080u) {
+            if (odd & kOdd) {
 #pragma unroll
                 for (int p = 0; p < kPasses; ++p) *reinterpret_cast<uint4*>(bs + p * (kRowsPerPass * 128)) = widen8_any<FMT>(c[p], k8[p]);
             }
