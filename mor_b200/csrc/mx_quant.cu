@@ -49,39 +49,45 @@ __device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t amax_bits) {
     return amax_bits >= 0x7F800000u ? 255u : byte;
 }
 
-// A lane owns eight consecutive elements, four lanes a group.  blockIdx.y walks the rows (one row where the matrix is
-// contiguous, whose groups then follow each other without a gap), blockIdx.x slices of a row.
-template <bool FP32, int U>
+// A lane owns eight consecutive elements, four lanes a group, a warp U times 256 elements in a row.  blockIdx.y walks the
+// rows (one row where the matrix is contiguous, whose groups then follow each other without a gap), blockIdx.x slices of
+// a row.  Bound by memory: all loads of a thread stand before their first use, U x 16 (32) bytes in flight each, and a
+// warp's scale bytes leave in one store.
+constexpr int kQU = 4;
+template <bool FP32>
 __global__ void __launch_bounds__(kQThreads) quantize_fp4_kernel(const void* __restrict__ in, uint32_t* __restrict__ payload,
                                                                  uint8_t* __restrict__ scales, int64_t rows, int64_t vec_per_row,
                                                                  int64_t pitch) {
+    const int lane = threadIdx.x & 31;
+    const int64_t first = (int64_t)blockIdx.x * (kQThreads * kQU) + (threadIdx.x >> 5) * (32 * kQU);
     pdl_wait();
     pdl_launch_dependents();
     for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
         const char* row = static_cast<const char*>(in) + r * pitch * (FP32 ? 4 : 2);
-        for (int64_t v0 = (int64_t)blockIdx.x * (kQThreads * U); v0 < vec_per_row; v0 += (int64_t)gridDim.x * (kQThreads * U)) {
-            float f[U][8];
-            uint4 w[U][FP32 ? 2 : 1];
+        for (int64_t v0 = first; v0 < vec_per_row; v0 += (int64_t)gridDim.x * (kQThreads * kQU)) {
+            uint4 w[kQU][FP32 ? 2 : 1];
+            uint32_t bytes = 0;   // of the group 8 u + lane % 8, for u = lane / 8
 #pragma unroll
-            for (int u = 0; u < U; ++u) {   // all loads of the thread before any use: U x 16 (32) bytes in flight
-                const int64_t v = v0 + u * kQThreads + threadIdx.x;
+            for (int u = 0; u < kQU; ++u) {
+                const int64_t v = v0 + u * 32 + lane;
                 const uint4* p = reinterpret_cast<const uint4*>(row + v * (FP32 ? 32 : 16));
                 w[u][0] = v < vec_per_row ? ld_stream(p) : make_uint4(0, 0, 0, 0);
                 if constexpr (FP32) w[u][1] = v < vec_per_row ? ld_stream(p + 1) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int64_t v = v0 + u * kQThreads + threadIdx.x;
+            for (int u = 0; u < kQU; ++u) {
+                const int64_t v = v0 + u * 32 + lane;
                 uint32_t amax;
+                float f[8];
                 if constexpr (FP32) {
                     const uint32_t a[8] = {w[u][0].x, w[u][0].y, w[u][0].z, w[u][0].w, w[u][1].x, w[u][1].y, w[u][1].z, w[u][1].w};
                     amax = 0;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) { f[u][i] = u2f(a[i]); amax = max(amax, a[i] & 0x7FFFFFFFu); }
+                    for (int i = 0; i < 8; ++i) { f[i] = u2f(a[i]); amax = max(amax, a[i] & 0x7FFFFFFFu); }
                 } else {
                     const uint32_t a[4] = {w[u][0].x, w[u][0].y, w[u][0].z, w[u][0].w};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) { f[u][2 * i] = bf16_lo(a[i]); f[u][2 * i + 1] = bf16_hi(a[i]); }
+                    for (int i = 0; i < 4; ++i) { f[2 * i] = bf16_lo(a[i]); f[2 * i + 1] = bf16_hi(a[i]); }
                     amax = hmax_halves(umax16x2_vec(mag2(a[0]), mag2(a[1]), mag2(a[2]), mag2(a[3]))) << 16;
                 }
                 amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
@@ -89,17 +95,16 @@ __global__ void __launch_bounds__(kQThreads) quantize_fp4_kernel(const void* __r
                 const uint32_t byte = fp4_scale_byte(amax);
                 const float up = u2f((254u - min(byte, 253u)) << 23);   // 2^(127 - byte), never subnormal: byte <= 253
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[u][i] = __fmul_rn(f[u][i], up);   // exact but for values far below the smallest code
-                const uint32_t codes = byte == 255u ? 0u : e2m1_codes8(f[u]);
-                if (v < vec_per_row) {
-                    const int64_t o = r * vec_per_row + v;
-                    payload[o] = codes;
-                    if ((threadIdx.x & 3) == 0) scales[o >> 2] = (uint8_t)byte;
-                }
+                for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], up);   // exact but for values far below the smallest code
+                if (v < vec_per_row) payload[r * vec_per_row + v] = byte == 255u ? 0u : e2m1_codes8(f);
+                const uint32_t mine = __shfl_sync(0xFFFFFFFFu, byte, (lane & 7) * 4);
+                bytes = (lane >> 3) == u ? mine : bytes;
             }
+            if (v0 + 4 * lane < vec_per_row) scales[((r * vec_per_row + v0) >> 2) + lane] = (uint8_t)bytes;
         }
     }
 }
+static_assert(kQU == 4, "a warp's 32 scale bytes, one a lane");
 
 // Two codes to two binary32 values: `c` holds two bytes (8-bit formats), or two nibbles (E2M1), the lower element low.
 template <int FMT>
@@ -171,11 +176,10 @@ inline unsigned grid_x(int64_t nvec, int per_cta) {
 int launch_quantize_fp4(const void* in, int is_fp32, int64_t rows, int64_t cols, int64_t pitch, void* payload, uint8_t* scales, cudaStream_t st) {
     int64_t r = rows, vpr = cols / 8;
     if (pitch == cols) { vpr *= r; r = 1; }
-    constexpr int U = 2;
-    const dim3 grid(grid_x(vpr, kQThreads * U), (unsigned)(r < 65535 ? r : 65535));
+    const dim3 grid(grid_x(vpr, kQThreads * kQU), (unsigned)(r < 65535 ? r : 65535));
     auto* p = static_cast<uint32_t*>(payload);
-    const cudaError_t e = is_fp32 ? launch_pdl(quantize_fp4_kernel<true, U>, grid, dim3(kQThreads), 0, st, in, p, scales, r, vpr, pitch)
-                                  : launch_pdl(quantize_fp4_kernel<false, U>, grid, dim3(kQThreads), 0, st, in, p, scales, r, vpr, pitch);
+    const cudaError_t e = is_fp32 ? launch_pdl(quantize_fp4_kernel<true>, grid, dim3(kQThreads), 0, st, in, p, scales, r, vpr, pitch)
+                                  : launch_pdl(quantize_fp4_kernel<false>, grid, dim3(kQThreads), 0, st, in, p, scales, r, vpr, pitch);
     return e == cudaSuccess ? check_launch() : kErrLaunch;
 }
 
