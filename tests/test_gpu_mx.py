@@ -168,7 +168,8 @@ def test_product_depths(m, k, fmt):
 
 @pytest.mark.parametrize("m,n,k,fmt", [(1, 4096, 4096, E2M1), (24, 4096, 8192, E4M3), (1111, 1003, 2080, E5M2), (2048, 2048, 2048, E2M1),
                                        (2500, 1536, 1024, E4M3), (2305, 1501, 608, E4M3), (2305, 1501, 608, E2M1), (1300, 2056, 32, E2M1),
-                                       (1300, 2056, 160, E5M2), (4096, 2048, 4128, E2M1), (4096, 300, 512, E2M1), (300, 4096, 512, E4M3)])
+                                       (1300, 2056, 160, E5M2), (4096, 2048, 4128, E2M1), (1300, 1400, 4096, E4M3), (1300, 1400, 8192, E2M1),
+                                       (2300, 2501, 4128, E4M3), (2300, 2504, 8224, E2M1), (1100, 1300, 16384, E5M2), (4096, 300, 512, E2M1), (300, 4096, 512, E4M3)])
 def test_product_sizes(m, n, k, fmt):
     check_product(m, n, k, fmt, fmt, bias=True)
 
@@ -212,7 +213,7 @@ def test_product_empty():
     assert z.shape == (4, 64) and not bool(z.any())
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 256, 4096), (40, 512, 4096), (600, 600, 1024), (2400, 2300, 1024)])
+@pytest.mark.parametrize("m,n,k", [(1, 256, 4096), (40, 512, 4096), (600, 600, 1024), (2400, 2300, 1024), (1300, 1400, 4096)])
 def test_product_repeats_bit_for_bit_on_any_stream(m, n, k):
     a, b, _ = product_case(m, n, k, E4M3, E4M3, 8, False)
     args = [t.cuda() for t in (*a, *b)]
@@ -307,7 +308,7 @@ def test_grad_depths(k, fmt, across):
 @pytest.mark.parametrize("across", [False, True])
 @pytest.mark.parametrize("m,n,k,fmt", [(1000, 2080, 1500, E4M3), (2048, 1024, 4096, E2M1), (4096, 4096, 33, E4M3), (20, 64, 8192, E5M2),
                                        (300, 32, 600, E4M3), (2500, 1056, 640, E2M1), (3000, 2080, 500, E4M3), (2304, 1312, 1000, E2M3),
-                                       (2568, 1312, 70, E5M2)])
+                                       (2568, 1312, 70, E5M2), (1300, 1408, 2500, E4M3), (2300, 2528, 4001, E2M1), (1304, 1408, 9000, E5M2)])
 def test_grad_sizes(m, n, k, fmt, across):
     check_grad(m, n, k, fmt, across)
 
@@ -349,7 +350,7 @@ def test_grad_nan_scale_and_strides():
 
 
 def test_grad_repeats_bit_for_bit():
-    for m, n, k in ((128, 128, 8192), (700, 1056, 1000)):
+    for m, n, k in ((128, 128, 8192), (700, 1056, 1000), (1304, 1408, 4000)):
         g = torch.randn(m, k, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
         c, s = (t.cuda() for t in R.random_codes(k, n, E4M3, 2))
         first = ops().mx_matmul_grad(g, c, s, m, n, k, 0, False)
