@@ -444,6 +444,72 @@ at::Tensor mx_matmul_grad(const at::Tensor& g, const at::Tensor& payload, const 
     return out;
 }
 
+// ---- a linear layer on microscaled operands -----------------------------------------------
+// Codes and scale bytes of a [rows, cols] tensor in groups of 32 columns; quantize_mx takes whole multiples of 256 elements.
+std::vector<at::Tensor> mx_quantized(const at::Tensor& x, int64_t format) {
+    const int64_t r = x.size(0), c = x.size(1);
+    if (format == MOR_B200_MX_E2M1) return quantize_mx_fp4(x, r, c, 32);
+    int64_t rows = 256;
+    for (int64_t d = c; rows > 1 && d % 2 == 0; d /= 2) rows /= 2;   // 256 / gcd(c, 256)
+    const int64_t padded = std::max((r + rows - 1) / rows, int64_t(1)) * rows;
+    if (padded == r) return quantize_mx(x, r, c, 32, format);
+    std::vector<at::Tensor> q = quantize_mx(at::constant_pad_nd(x, {0, 0, 0, padded - r}), padded, c, 32, format);
+    return {q[0].narrow(0, 0, r), q[1].narrow(0, 0, r)};
+}
+
+// Straight-through: the gradients are those of a linear layer fed the quantised values, computed from the codes, which are
+// all that the forward pass keeps of the input and the weight.
+struct MxLinear : public torch::autograd::Function<MxLinear> {
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
+                              const std::optional<at::Tensor>& bias, int64_t format) {
+        const int64_t k = weight.size(1), n = weight.size(0);
+        at::Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, k});
+        const int64_t m = x2.size(0);
+        const std::vector<at::Tensor> xq = mx_quantized(x2, format), wq = mx_quantized(weight, format);
+        std::optional<at::Tensor> b;
+        if (bias.has_value() && bias->defined()) b = bias->scalar_type() == at::kBFloat16 ? *bias : bias->to(at::kBFloat16);
+        at::Tensor y = mx_matmul(xq[0], xq[1], wq[0], wq[1], m, n, k, format, format, b);
+        const bool need_x = x.requires_grad(), need_w = weight.requires_grad();
+        ctx->save_for_backward({need_x ? wq[0] : at::Tensor(), need_x ? wq[1] : at::Tensor(), need_w ? xq[0] : at::Tensor(),
+                                need_w ? xq[1] : at::Tensor()});
+        ctx->saved_data["format"] = format;
+        ctx->saved_data["x_sizes"] = x.sizes().vec();
+        ctx->saved_data["n"] = n;
+        ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)x.scalar_type(), (int64_t)weight.scalar_type(),
+                                                        b.has_value() ? (int64_t)bias->scalar_type() : 0};
+        if (x.dim() == 2) return y;
+        std::vector<int64_t> shape = x.sizes().vec();
+        shape.back() = n;
+        return y.reshape(shape);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "mor::mx_linear is differentiable once: its gradients have no gradient (create_graph)");
+        const torch::autograd::variable_list kept = ctx->get_saved_variables();
+        const int64_t format = ctx->saved_data["format"].toInt(), n = ctx->saved_data["n"].toInt();
+        const std::vector<int64_t> sizes = ctx->saved_data["x_sizes"].toIntVector(), types = ctx->saved_data["types"].toIntVector();
+        const int64_t k = sizes.back();
+        at::Tensor g = grads[0].dim() == 2 ? grads[0] : grads[0].reshape({-1, n});
+        const int64_t m = g.size(0);
+        auto typed = [](at::Tensor t, int64_t type) { return t.scalar_type() == (at::ScalarType)type ? t : t.to((at::ScalarType)type); };
+        at::Tensor gx, gw, gb;
+        if (kept[0].defined()) {
+            gx = typed(mx_matmul_grad(g, kept[0], kept[1], m, k, n, format, false), types[0]);
+            if (sizes.size() != 2) gx = gx.reshape(sizes);
+        }
+        if (kept[2].defined()) gw = typed(mx_matmul_grad(g, kept[2], kept[3], n, k, m, format, true), types[1]);
+        if (types[2] && ctx->needs_input_grad(2)) gb = typed(g.sum(0), types[2]);
+        return {gx, gw, gb, at::Tensor()};
+    }
+};
+
+at::Tensor mx_linear(const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& bias, int64_t format) {
+    TORCH_CHECK(x.is_cuda() && weight.device() == x.device(), "mor::mx_linear: x and weight must be CUDA tensors on one device");
+    TORCH_CHECK(format == MOR_B200_E4M3 || format == MOR_B200_E5M2 || format == MOR_B200_MX_E2M1,
+                "mor::mx_linear: elem_format must be 0 (E4M3), 1 (E5M2) or 4 (E2M1)");
+    TORCH_CHECK(weight.dim() == 2 && x.dim() >= 1 && x.size(-1) == weight.size(1), "mor::mx_linear: x must be [..., in] and weight [out, in]");
+    return MxLinear::apply(x, weight, bias, format);
+}
+
 }  // namespace
 
 // Registers _C as a Python extension module.
@@ -477,6 +543,7 @@ TORCH_LIBRARY(mor, m) {
   m.def("dequantize_mx(Tensor payload, Tensor scales, int dim_x, int dim_y, int block_y, int elem_format, ScalarType out_dtype) -> Tensor");
   m.def("mx_matmul(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, int dim_m, int dim_n, int dim_k, int a_format, int b_format, Tensor? bias) -> Tensor");
   m.def("mx_matmul_grad(Tensor g, Tensor payload, Tensor scales, int dim_m, int dim_n, int dim_k, int elem_format, bool transpose_g) -> Tensor");
+  m.def("mx_linear(Tensor x, Tensor weight, Tensor? bias, int elem_format) -> Tensor", &mx_linear);   // composed of the above, with its gradient
 }
 
 TORCH_LIBRARY_IMPL(mor, CUDA, m) {

@@ -195,43 +195,12 @@ def _mx_quantize(x: Tensor, elem_format: int):
     r, c = x.shape
     if elem_format == 4:
         return ops.quantize_mx_fp4(x, r, c, 32)
-    short = -r % (256 // math.gcd(c, 256))      # quantize_mx takes whole multiples of 256 elements
-    if short or r == 0:
-        short = short or 256 // math.gcd(c, 256)
-        codes, scales = ops.quantize_mx(torch.nn.functional.pad(x, (0, 0, 0, short)), r + short, c, 32, elem_format)
-        return codes[:r], scales[:r]
-    return ops.quantize_mx(x, r, c, 32, elem_format)
-
-
-class _MXLinearFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x: Tensor, weight: Tensor, bias: Optional[Tensor], elem_format: int) -> Tensor:
-        x2 = x.reshape(-1, x.shape[-1])
-        xc, xs = _mx_quantize(x2, elem_format)
-        wc, ws = _mx_quantize(weight, elem_format)
-        m, n, k = x2.shape[0], weight.shape[0], weight.shape[1]
-        y = ops.mx_matmul(xc, xs, wc, ws, m, n, k, elem_format, elem_format, None if bias is None else bias.to(torch.bfloat16))
-        need_x, need_w = ctx.needs_input_grad[:2]
-        # what the backward pass reads is the codes: 8 (4) bits an element and a scale byte per 32
-        ctx.save_for_backward(*((wc, ws) if need_x else (None, None)), *((xc, xs) if need_w else (None, None)))
-        ctx.elem_format, ctx.sizes, ctx.x_shape = elem_format, (m, n, k), x.shape
-        ctx.types = (x.dtype, weight.dtype, None if bias is None else bias.dtype)
-        return y.reshape(*x.shape[:-1], n)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad: Tensor):
-        wc, ws, xc, xs = ctx.saved_tensors
-        m, n, k = ctx.sizes
-        g = grad.reshape(m, n)
-        gx = gw = gb = None
-        if ctx.needs_input_grad[0]:
-            gx = ops.mx_matmul_grad(g, wc, ws, m, k, n, ctx.elem_format, False).to(ctx.types[0]).reshape(ctx.x_shape)
-        if ctx.needs_input_grad[1]:
-            gw = ops.mx_matmul_grad(g, xc, xs, n, k, m, ctx.elem_format, True).to(ctx.types[1])
-        if ctx.needs_input_grad[2]:
-            gb = g.sum(0).to(ctx.types[2])
-        return gx, gw, gb, None
+    whole = 256 // math.gcd(c, 256)             # quantize_mx takes whole multiples of 256 elements
+    padded = max(-(-r // whole), 1) * whole
+    if padded == r:
+        return ops.quantize_mx(x, r, c, 32, elem_format)
+    codes, scales = ops.quantize_mx(torch.nn.functional.pad(x, (0, 0, 0, padded - r)), padded, c, 32, elem_format)
+    return codes[:r], scales[:r]
 
 
 def mx_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, elem_format: int = 0) -> Tensor:
@@ -239,13 +208,14 @@ def mx_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, elem_for
     groups of 32 along ``in`` (a multiple of 32) and multiplied as codes; the result is bfloat16.  ``elem_format``: 0 E4M3,
     1 E5M2 (bfloat16 inputs), 4 E2M1 (bfloat16 or float32).  The gradients are straight-through: those of a linear layer
     fed the quantised values, computed from the codes, which are all that the forward pass keeps of ``x`` and ``weight``
-    -- one byte (E2M1: half a byte) and a thirty-second per element in place of two.  Each call quantises the weight it
+    -- one byte (E2M1: half a byte) and a thirty-second per element in place of two; they have no gradient of their own.
+    Each call quantises the weight it
     is given; for serving see :meth:`MXLinear.pack`."""
     if elem_format not in MX_FORMATS.values():
         raise ValueError(f"elem_format must be one of {sorted(MX_FORMATS.values())}, got {elem_format}")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"x [..., in] and weight [out, in] expected, got {tuple(x.shape)} and {tuple(weight.shape)}")
-    return _MXLinearFunction.apply(x, weight, bias, elem_format)
+    return torch.ops.mor.mx_linear.default(x, weight, bias, elem_format)
 
 
 class MXLinear(torch.nn.Linear):

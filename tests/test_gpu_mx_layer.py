@@ -172,6 +172,31 @@ def test_captured_step_replays_with_new_values():
     assert all(torch.equal(u, v) for u, v in zip(outs, want)) and all(torch.equal(u, v) for u, v in zip(outs2, want))
 
 
+def test_gradients_have_no_gradient():
+    from mor_b200.nn import mx_linear
+    x = torch.randn(8, 32, device="cuda").to(torch.bfloat16).requires_grad_()
+    w = torch.randn(8, 32, device="cuda").to(torch.bfloat16).requires_grad_()
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(mx_linear(x, w).float().square().sum(), x, create_graph=True)
+    with torch.no_grad():
+        assert not mx_linear(x, w).requires_grad
+
+
+def test_layer_refusals():
+    from mor_b200.nn import mx_linear
+    x = torch.randn(8, 32, device="cuda").to(torch.bfloat16)
+    with pytest.raises(ValueError):
+        mx_linear(x, x[:, :16])
+    with pytest.raises(RuntimeError, match="one device"):
+        mx_linear(x, x.cpu())
+    with pytest.raises(RuntimeError, match="bfloat16"):
+        mx_linear(x.float(), x, None, 0)             # the 8-bit quantiser takes bfloat16
+    with pytest.raises(RuntimeError, match="multiple of 32"):
+        mx_linear(x[:, :24].contiguous(), x[:, :24].contiguous(), None, 4)
+    with pytest.raises(RuntimeError, match="bias"):
+        mx_linear(x, x, torch.zeros(3, device="cuda", dtype=torch.bfloat16), 4)
+
+
 def test_training_runs():
     from mor_b200.nn import MXLinear
     torch.manual_seed(0)
