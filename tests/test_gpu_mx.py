@@ -357,6 +357,50 @@ def test_grad_repeats_bit_for_bit():
         assert all(torch.equal(first, ops().mx_matmul_grad(g, c, s, m, n, k, 0, False)) for _ in range(4))
 
 
+def test_gradient_rows_beyond_the_result_are_left_alone():
+    from mor_b200 import cabi
+    for m, n, k in ((5, 64, 40), (133, 160, 70), (300, 96, 4096), (2309, 1312, 100)):
+        g = torch.randn(m, (k + 7) // 8 * 8, device="cuda").to(torch.bfloat16)
+        c, s = (t.cuda() for t in R.random_codes(k, n, E4M3, 2))
+        out = torch.full((m * n + 4096,), 7.0, dtype=torch.bfloat16, device="cuda")
+        cabi.call("mor_b200_mx_matmul_grad", g.data_ptr(), g.shape[1], c.data_ptr(), s.data_ptr(), m, n, k, 0, 0, out.data_ptr(),
+                  torch.cuda.current_stream().cuda_stream)
+        assert bool((out[m * n:] == 7.0).all())
+        assert torch.equal(out[:m * n].view(m, n), ops().mx_matmul_grad(g[:, :k], c, s, m, n, k, 0, False))
+
+
+# ------------------------------------------------------------------------------------------------ more than 2^31 elements
+def test_quantisation_past_32_bits():
+    r, c = 70000, 32768
+    x = torch.zeros(r, c, dtype=torch.bfloat16, device="cuda")
+    at = [0, 1, r // 2, r - 2, r - 1]
+    x[at] = torch.randn(len(at), c, device="cuda").to(torch.bfloat16)
+    p, s = ops().quantize_mx_fp4(x, r, c, 32)
+    ep, es = R.quantize_fp4(x[at].double().cpu().numpy())
+    assert torch.equal(p[at].cpu(), ep) and torch.equal(s[at].cpu(), es)
+    del x
+    y = ops().dequantize_mx(p, s, r, c, 32, E2M1)
+    assert torch.equal(y[at].double().cpu(), R.decode(ep, es, E2M1))
+    assert int((y != 0).sum(dtype=torch.int64)) == int((y[at] != 0).sum())
+
+
+def test_products_past_32_bits():
+    m, n, k = 66000, 33000, 32
+    a, b = R.random_codes(m, k, E4M3, 1), R.random_codes(n, k, E4M3, 2)
+    y = ops().mx_matmul(a[0].cuda(), a[1].cuda(), b[0].cuda(), b[1].cuda(), m, n, k, 0, 0)
+    va, vb = R.decode(*a, E4M3).cuda(), R.decode(*b, E4M3).cuda()
+    for rows in (slice(0, 3), slice(m - 300, m)):
+        exact, size = va[rows] @ vb.t(), va[rows].abs() @ vb.abs().t()
+        close(y[rows], exact.cpu(), size.cpu(), k, 32)
+    del y, va, vb
+    n = 32800                       # the same from a gradient, whose outputs are a multiple of 32 wide
+    g = torch.randn(m, 16, device="cuda").to(torch.bfloat16)
+    w = R.random_codes(16, n, E2M1, 3)
+    y = ops().mx_matmul_grad(g, w[0].cuda(), w[1].cuda(), m, n, 16, E2M1, False)
+    gd, wd = g[-300:].double().cpu(), R.decode(*w, E2M1)
+    close(y[-300:], gd @ wd, gd.abs() @ wd.abs(), 16, 16)
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def test_refusals():
     o = ops()
