@@ -7,6 +7,7 @@
 // torch::empty on the input's device, and launches on the CURRENT stream (the
 // reference uses the legacy default stream).  It holds no arithmetic.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -336,6 +337,10 @@ std::vector<at::Tensor> quantize_scaled(const at::Tensor& input, int64_t rows, i
 
 // ---- extension: microscaled operands (include/mor_b200_mx.h) -----------------------------
 // One code per element, or two to a byte for E2M1; the tensors of one operand lie on one device.
+// Outputs of these operators are taken from the allocator directly: the calls for single tokens are as long as their host side.
+at::Tensor mx_empty(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& like) {
+    return at::Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt));
+}
 bool mx_format_ok(int64_t f) { return f == MOR_B200_E4M3 || f == MOR_B200_E5M2 || f == MOR_B200_E2M3 || f == MOR_B200_MX_E2M1; }
 
 at::Tensor mx_part(const at::Tensor& t, int64_t rows, int64_t cols, const at::Tensor& like, size_t align, const char* op, const char* what) {
@@ -356,7 +361,7 @@ at::Tensor mx_rows(const at::Tensor& t, int64_t& pitch) {
     const bool unit = t.stride(1) == 1 || t.size(1) == 1;
     if (unit && pitch >= t.size(1) && pitch * w % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) return t;
     pitch = packed;
-    at::Tensor p = torch::empty({t.size(0), packed}, t.options());
+    at::Tensor p = mx_empty({t.size(0), packed}, t.scalar_type(), t);
     p.narrow(1, 0, t.size(1)).copy_(t);
     return p;
 }
@@ -370,8 +375,8 @@ std::vector<at::Tensor> quantize_mx_fp4(const at::Tensor& input, int64_t rows, i
     const int dt = dtype_code(input, true, "quantize_mx_fp4");
     TORCH_CHECK(bc == 32, "mor::quantize_mx_fp4: block_y must be 32");
     TORCH_CHECK(cols > 0 && cols % 32 == 0, "mor::quantize_mx_fp4: dim_y must be a positive multiple of 32");
-    at::Tensor payload = torch::empty({rows, cols / 2}, input.options().dtype(torch::kUInt8));
-    at::Tensor scales = torch::empty({rows, cols / 32}, input.options().dtype(torch::kUInt8));
+    at::Tensor payload = mx_empty({rows, cols / 2}, at::kByte, input);
+    at::Tensor scales = mx_empty({rows, cols / 32}, at::kByte, input);
     if (rows == 0) return {payload, scales};
     int64_t pitch = 0;
     at::Tensor in = mx_rows(input, pitch);
@@ -390,7 +395,7 @@ at::Tensor dequantize_mx(const at::Tensor& payload, const at::Tensor& scales, in
                 "mor::dequantize_mx: block_y must be a power of two from 8 to 256 that divides dim_y");
     at::Tensor p = mx_payload(payload, rows, cols, format, payload, "dequantize_mx", "payload");
     at::Tensor s = mx_part(scales, rows, cols / bc, payload, 1, "dequantize_mx", "scales");
-    at::Tensor out = torch::empty({rows, cols}, payload.options().dtype(dtype));
+    at::Tensor out = mx_empty({rows, cols}, dtype, payload);
     check_status(mor_b200_mx_dequantize(p.data_ptr(), s.data_ptr(), out.data_ptr(), dtype == at::kFloat ? MOR_B200_FP32 : MOR_B200_BF16,
                                         rows, cols, (int)bc, (int)format, cur_stream()),
                  "dequantize_mx");
@@ -413,10 +418,10 @@ at::Tensor mx_matmul(const at::Tensor& a, const at::Tensor& a_scales, const at::
                     "mor::mx_matmul: bias must be bfloat16 [dim_n] on ", a.device());
         bi = bias->contiguous();
     }
-    at::Tensor out = torch::empty({m, n}, a.options().dtype(torch::kBFloat16));
+    at::Tensor out = mx_empty({m, n}, at::kBFloat16, a);
     const size_t wsb = mor_b200_mx_matmul_workspace_bytes(m, n, k);
     at::Tensor ws;
-    if (wsb) ws = workspace(a, wsb);
+    if (wsb) ws = mx_empty({(int64_t)wsb}, at::kByte, a);
     check_status(mor_b200_mx_matmul(ac.data_ptr(), as.data_ptr(), bcod.data_ptr(), bs.data_ptr(), m, n, k, (int)a_format, (int)b_format,
                                     bi.defined() ? bi.data_ptr() : nullptr, out.data_ptr(), wsb ? ws.data_ptr() : nullptr, wsb, cur_stream()),
                  "mx_matmul");
@@ -434,7 +439,7 @@ at::Tensor mx_matmul_grad(const at::Tensor& g, const at::Tensor& payload, const 
                 "mor::mx_matmul_grad: g must be [dim_m, dim_k], or [dim_k, dim_m] with transpose_g");
     at::Tensor p = mx_payload(payload, k, n, format, g, "mx_matmul_grad", "payload");
     at::Tensor s = mx_part(scales, k, n / 32, g, 1, "mx_matmul_grad", "scales");
-    at::Tensor out = torch::empty({m, n}, g.options());
+    at::Tensor out = mx_empty({m, n}, at::kBFloat16, g);
     if (m == 0 || n == 0) return out;
     int64_t pitch = 0;
     at::Tensor gr = mx_rows(g, pitch);
