@@ -3,6 +3,12 @@
 // Both operands are K-major with one E8M0 byte for every 32 elements of a row, which is what the instruction multiplies
 // into the product itself: the codes go from global to shared memory by TMA and are never widened.  A tile is 128 rows of
 // one operand (P) by TN rows of the other (Q), 128 bytes of K (256 E2M1 or 128 E4M3 / E5M2 elements) at a time.
+//
+// The tensor core takes such a step of a 256 x 256 tile in 0.287 us (4.3 PFLOP/s 8-bit, 8.6 4-bit over 148 SMs), so a
+// kernel of this kind lives by handing it operands without a pause.  Measured: 8192^3 4-bit 190 us in a short run (5.8
+// PFLOP/s, tensor pipe 82 % active), 225 us in a long one, where the card's power limit lowers the clock; 8192 x 4096 x
+// 4096 E4M3 103 and 122 us (74 %).  Few tokens are bound by reading the weights: 24 x 16384 x 8192 E4M3 27 us (5.1 TB/s);
+// one token x 4096 x 4096 4-bit by latency, 5.4 us.
 #include <algorithm>
 
 #include "mx_kernels.cuh"
@@ -292,6 +298,8 @@ struct PairShape {
     static_assert(kSmem <= 227 * 1024 - 2048, "shared memory");
 };
 
+// Each operand byte crosses from L2 once for 256 rows of the other operand (11 to 13 TB/s for the whole card at the rates
+// above; single CTAs on 128 x 128 need twice that and take 290 us where pairs take 103).
 // Warps 0-7 write the results, warp 8 loads, warp 9 issues (in the first CTA) or says that this CTA's operands are there
 // (in the second).  Each CTA loads 128 rows of either operand, A's scales for its rows and B's for all 256 columns.  The
 // accumulator fills half of tensor memory and the scales need some of the rest, so there is one: between two tiles the

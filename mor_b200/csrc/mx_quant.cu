@@ -51,8 +51,9 @@ __device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t amax_bits) {
 
 // A lane owns eight consecutive elements, four lanes a group, a warp U times 256 elements in a row.  blockIdx.y walks the
 // rows (one row where the matrix is contiguous, whose groups then follow each other without a gap), blockIdx.x slices of
-// a row.  Bound by memory: all loads of a thread stand before their first use, U x 16 (32) bytes in flight each, and a
-// warp's scale bytes leave in one store.
+// a row.  Bound by memory, with the integer pipe close behind (72 %): all loads of a thread stand before their first use,
+// four of 16 (32) bytes in flight each (8192^2 bf16: two take 34.0 us, four 30.4, eight 30.2), and a warp's scale bytes
+// leave in one store (29.1 us = 5.8 TB/s; 1003 x 4128 float32 out of wider rows 5.0 us).
 constexpr int kQU = 4;
 template <bool FP32>
 __global__ void __launch_bounds__(kQThreads) quantize_fp4_kernel(const void* __restrict__ in, uint32_t* __restrict__ payload,
@@ -118,7 +119,8 @@ __device__ __forceinline__ void decode2(uint32_t c, float& lo, float& hi) {
 
 // A lane writes 16 bytes: eight bf16 or four binary32 values.  value = decode(code) * 2^(scale - 127) is exact in
 // binary32 (at most four significant bits, nothing below 2^-143), so the one rounding is the one to bf16, to nearest
-// even, and only subnormal results meet it.
+// even, and only subnormal results meet it.  Bound by memory: 16384 x 8192 E4M3 to bf16 61.5 us = 6.6 TB/s, 8192^2 E2M1
+// 27.0 us = 6.3 TB/s (two loads of codes in flight a thread 30.2, four 27.0, eight 27.9).
 template <int FMT, bool FP32, int U>
 __global__ void __launch_bounds__(kQThreads) dequantize_kernel(const uint8_t* __restrict__ payload, const uint8_t* __restrict__ scales,
                                                                uint4* __restrict__ out, int64_t nvec, int log2_group) {
