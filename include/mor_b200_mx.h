@@ -44,15 +44,15 @@ MOR_B200_MX_API int mor_b200_mx_dequantize(const void* payload, const void* scal
                                            int64_t cols, int block_cols, int format, void* stream);
 
 /* out[m, n] = sum_k A[m, k] B[n, k] (+ bias[n]): both operands MX with groups of 32 along k, k a positive multiple of 32,
- * payloads 16-byte and scales 4-byte aligned.  Formats: both E2M1, or each E4M3 or E5M2.  bias: bf16 [n] or NULL; out:
+ * payloads and scales 16-byte aligned.  Formats: both E2M1, or each E4M3 or E5M2.  bias: bf16 [n] or NULL; out:
  * bf16 [m, n], 2-byte aligned.  Products and sums are formed by the tensor core in binary32, the bias is added in
  * binary32, and the result is rounded once.  m <= 64 takes a form in which tokens fill a narrow tile.  Sums that are
  * split over the CTAs of a cluster are added in a fixed order: results repeat bit for bit.
- * Some products (m above 64, k not a multiple of 128) need a workspace of
- * mor_b200_mx_matmul_workspace_bytes(m, n, k) bytes (0 for the others, which take NULL), 16-byte aligned, of any content.
+ * Large products need a workspace of mor_b200_mx_matmul_workspace_bytes(m, n, k, a_format) bytes (0 for the others, which
+ * take NULL), 16-byte aligned, of any content.
  * Scale bytes lie in it in tensor-core order while the call runs, so calls that may overlap (other streams, captured
  * graphs) need one each. */
-MOR_B200_MX_API size_t mor_b200_mx_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k);
+MOR_B200_MX_API size_t mor_b200_mx_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, int a_format);
 MOR_B200_MX_API int mor_b200_mx_matmul(const void* a, const void* a_scales, const void* b, const void* b_scales, int64_t m,
                                        int64_t n, int64_t k, int a_format, int b_format, const void* bias, void* out,
                                        void* workspace, size_t workspace_bytes, void* stream);

@@ -43,9 +43,9 @@ int mor_b200_mx_dequantize(const void* payload, const void* scales, void* out, i
                              static_cast<cudaStream_t>(stream));
 }
 
-size_t mor_b200_mx_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+size_t mor_b200_mx_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, int a_format) {
     if (m <= 0 || n <= 0 || k <= 0 || k % 32 || too_large(m) || too_large(n) || too_large(k)) return 0;
-    return mx_matmul_workspace(m, n, k);
+    return mx_matmul_workspace(m, n, k, a_format == kE2M1);
 }
 
 int mor_b200_mx_matmul(const void* a, const void* a_scales, const void* b, const void* b_scales, int64_t m, int64_t n, int64_t k,
@@ -58,9 +58,9 @@ int mor_b200_mx_matmul(const void* a, const void* a_scales, const void* b, const
     if (m == 0 || n == 0) return kOk;
     if (!a || !a_scales || !b || !b_scales || !out) return kErrInvalidArgument;
     if (too_large(m) || too_large(n) || too_large(k)) return kErrTooLarge;
-    if (!aligned(a, 16) || !aligned(b, 16) || !aligned(a_scales, 4) || !aligned(b_scales, 4) || !aligned(out, 2) || !aligned(bias, 2))
+    if (!aligned(a, 16) || !aligned(b, 16) || !aligned(a_scales, 16) || !aligned(b_scales, 16) || !aligned(out, 2) || !aligned(bias, 2))
         return kErrUnsupportedShape;
-    const size_t need = mx_matmul_workspace(m, n, k);
+    const size_t need = mx_matmul_workspace(m, n, k, fp4);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return kErrWorkspace;
     const MxMatmulArgs x{a, b, static_cast<const uint8_t*>(a_scales), static_cast<const uint8_t*>(b_scales), bias, out, m, n, k, a_format, b_format, workspace};
     return launch_mx_matmul(x, static_cast<cudaStream_t>(stream));

@@ -22,7 +22,7 @@ struct MxMatmulArgs {
     int a_fmt, b_fmt;
     void* workspace;    // mx_matmul_workspace bytes
 };
-size_t mx_matmul_workspace(int64_t m, int64_t n, int64_t k);
+size_t mx_matmul_workspace(int64_t m, int64_t n, int64_t k, int fp4);
 int launch_mx_matmul(const MxMatmulArgs& a, cudaStream_t st);
 
 // mx_grad.cu: out[m, n] = sum_k op(g)[m, k] decode(payload)[k, n]

@@ -26,7 +26,7 @@ struct MmArgs {
     int64_t ldo;              // row pitch of out (= n)
     int64_t p_tiles;
     uint32_t idesc;
-    int ktiles, splits, tiled_scales, vec_out;
+    int ktiles, splits, vec_out;
 };
 
 constexpr int kPRows = 128;
@@ -46,25 +46,58 @@ struct MmShape {
     static_assert(kSmem > 114 * 1024, "one CTA per SM");
 };
 
-// Scale bytes of one row for one step: four a block, to the place the tensor core's copy takes them from (row r of 128:
-// 16 bytes for each r mod 32, four for each r / 32).  Rows and groups outside read as zero, a finite scale.  The bytes of
-// a block lie on four bytes: groups is a multiple of four here.
-template <int BLK>
-__device__ __forceinline__ void load_scales(uint32_t dst, const uint8_t* s, int64_t row, int64_t rows, int64_t groups, int64_t g0) {
+// Scale bytes of a row for the next kBatch steps, W words of four, wherever they lie: 16-byte loads that cover them (no
+// byte outside the tensor is read), moved into place when they are used, so that a batch can be in flight while the one
+// before is stored.  A step's words go to the places the tensor core's copy takes them from (512 bytes for four groups of 128
+// rows: 16 for each row mod 32, four for each row / 32); rows and groups outside read as zero, a finite scale.
+constexpr int kBatch = 4;
+template <int W>
+struct ScaleWords {
+    static constexpr int kChunks = W / 4 + 1;
+    uint32_t x[4 * kChunks];
+    int offset, valid;   // of the first byte in the first chunk; groups left in the row
+    __device__ __forceinline__ void load(const uint8_t* s, int64_t rows, int64_t groups, int64_t row, int64_t g0) {
+        const int64_t o = row * groups + g0, total = rows * groups, left = groups - g0;
+        valid = row < rows && left > 0 ? (int)(left < 4 * W ? left : 4 * W) : 0;
+        offset = (int)(o & 15);
 #pragma unroll
-    for (int b = 0; b < BLK; ++b) {
-        const int64_t g = g0 + 4 * b;
-        const bool in = row < rows && g < groups;
-        cp_async4(dst + b * 512, s + (in ? row * groups + g : 0), in ? 4 : 0);
+        for (int c = 0; c < kChunks; ++c) {
+            const int64_t at = o - offset + 16 * c;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (offset + valid > 16 * c && valid > 0) {
+                if (at + 16 <= total) {
+                    v = __ldg(reinterpret_cast<const uint4*>(s + at));
+                } else {   // the tensor's last bytes
+                    uint32_t w[4] = {};
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (at + e < total) w[e >> 2] |= (uint32_t)__ldg(s + at + e) << (8 * (e & 3));
+                    v = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            x[4 * c] = v.x; x[4 * c + 1] = v.y; x[4 * c + 2] = v.z; x[4 * c + 3] = v.w;
+        }
     }
-}
+    __device__ __forceinline__ void place(uint32_t (&w)[W]) {
+        constexpr int n = 4 * kChunks;
+#pragma unroll
+        for (int j = 0; j < n - 2; ++j) x[j] = offset & 8 ? x[j + 2] : x[j];
+#pragma unroll
+        for (int j = 0; j < n - 3; ++j) x[j] = offset & 4 ? x[j + 1] : x[j];
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const int left = valid - 4 * j;
+            w[j] = __funnelshift_r(x[j], x[j + 1], 8 * (offset & 3));
+            w[j] = left >= 4 ? w[j] : (left <= 0 ? 0u : w[j] & ((1u << (8 * left)) - 1u));
+        }
+    }
+};
+__device__ __forceinline__ void store_word(uint32_t dst, uint32_t w) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst), "r"(w) : "memory"); }
 
 // SWAP: P is B (rows of out's columns) and Q is A, so that few tokens fill a narrow tile of many weight rows.
-// Warps 0-3 fetch scale bytes (unless a kernel ahead has put them in order, then warp 4 does) and write the result, warp 4
-// loads, warp 5 issues.
+// Warps 0-3 fetch scale bytes and then write the result, warp 4 loads codes, warp 5 issues.
 template <bool FP4, int TN, bool SWAP>
 __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
-                                                           const __grid_constant__ CUtensorMap map_sp, const __grid_constant__ CUtensorMap map_sq,
                                                            const MmArgs a) {
     using S = MmShape<FP4, TN>;
     constexpr int kGroupsPerStep = FP4 ? 8 : 4;
@@ -81,7 +114,7 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
     const int n = k_last - k_first;
 
     if (warp == 4 && lane == 0) {
-        for (int s = 0; s < S::kStages; ++s) { mbar_init(&full[s], a.tiled_scales ? 1 : 1 + 128); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(&full[s], 1 + 4); mbar_init(&empty[s], 1); }
         mbar_init(&acc_done, 1);
         mbar_init(&drained, 1);
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_p));
@@ -105,13 +138,9 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
                 uint8_t* st = smem + sl.s * S::kStage;
                 uint64_t* bar = &full[sl.s];
                 const int x = (k_first + i) * 128;
-                mbar_expect_tx(bar, S::kPBytes + S::kQBytes + (a.tiled_scales ? (S::kBlk + S::kQBlk) * 512 : 0));
+                mbar_expect_tx(bar, S::kPBytes + S::kQBytes);
                 tma_load_2d(st, &map_p, x, (int)p0, bar);
                 tma_load_2d(st + S::kPBytes, &map_q, x, (int)q0, bar);
-                if (a.tiled_scales) {
-                    tma_load_2d(st + S::kSfOff, &map_sp, x * S::kBlk, (int)tp, bar);   // 128 words a block
-                    tma_load_2d(st + S::kSfOff + S::kBlk * 512, &map_sq, x * S::kBlk, (int)(q0 / 128), bar);
-                }
             }
             __syncwarp();
             sl.advance();
@@ -126,7 +155,6 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
-                fence_async_shared();   // scale bytes that came by ordinary copies; the tensor core reads through its own path
                 const uint32_t sf = smem_u32(smem) + sl.s * S::kStage + S::kSfOff;
                 const uint32_t sfp = tmem + TN + (i & 1) * S::kSfCols, sfq = sfp + 4 * S::kBlk;
 #pragma unroll
@@ -149,21 +177,41 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
             mbar_wait_bounded(&drained, 0);
         }
     } else {
-        if (!a.tiled_scales) {
-            const int t = threadIdx.x;   // 0..127
-            const uint32_t place = (t & 31) * 16 + (t >> 5) * 4;
-            Slot<S::kStages> sl;
-            for (int i = 0; i < n; ++i) {
+        const int t = threadIdx.x;   // 0..127
+        const uint32_t sf = smem_u32(smem) + S::kSfOff + (t & 31) * 16 + (t >> 5) * 4;
+        constexpr int W = kBatch * S::kBlk;
+        Slot<S::kStages> sl;
+        ScaleWords<W> p, q, next_p, next_q;
+        const int64_t g0 = (int64_t)k_first * kGroupsPerStep;
+        const bool has_q = warp < (TN + 31) / 32;
+        p.load(a.sp, a.p_rows, a.groups, p0 + t, g0);
+        if (has_q) q.load(a.sq, a.q_rows, a.groups, q0 + t, g0);
+        for (int i = 0; i < n && ok; i += kBatch) {
+            if (i + kBatch < n) {
+                next_p.load(a.sp, a.p_rows, a.groups, p0 + t, g0 + (int64_t)(i + kBatch) * kGroupsPerStep);
+                if (has_q) next_q.load(a.sq, a.q_rows, a.groups, q0 + t, g0 + (int64_t)(i + kBatch) * kGroupsPerStep);
+            }
+            uint32_t wp[W], wq[W];
+            p.place(wp);
+            if (has_q) q.place(wq);
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                if (i + u >= n) break;
                 ok = mbar_wait_warp(&empty[sl.s], sl.phase ^ 1);
                 if (!ok) break;
-                const uint32_t sf = smem_u32(smem + sl.s * S::kStage + S::kSfOff) + place;
-                const int64_t g0 = (int64_t)(k_first + i) * kGroupsPerStep;
-                load_scales<S::kBlk>(sf, a.sp, p0 + t, a.p_rows, a.groups, g0);
-                if (t < TN) load_scales<S::kBlk>(sf + 512 * S::kBlk, a.sq, q0 + t, a.q_rows, a.groups, g0);
-                cp_async_arrive(&full[sl.s]);
+                const uint32_t to = sf + sl.s * S::kStage;
+#pragma unroll
+                for (int b = 0; b < S::kBlk; ++b) {
+                    store_word(to + 512 * b, wp[u * S::kBlk + b]);
+                    if (has_q) store_word(to + 512 * (S::kBlk + b), wq[u * S::kBlk + b]);
+                }
+                fence_async_shared();
+                __syncwarp();
+                if (elect_one()) mbar_arrive(&full[sl.s]);
                 sl.advance();
             }
-            cp_async_wait_all();
+            p = next_p;
+            q = next_q;
         }
         ok = ok && mbar_wait_warp(&acc_done, 0);
         tc_fence_after();
@@ -249,7 +297,7 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
 // ---------------------------------------------------------------------------------
 // Scale bytes [rows, groups] in the order the tensor core's copy wants them: for every 128 rows and four groups 512 bytes,
 // 16 for each r mod 32, four for each r / 32, zeros where there is no row or group.  One thread takes 16 groups of a row.
-__global__ void __launch_bounds__(128) tile_scales_kernel(const uint8_t* __restrict__ sa, int64_t rows_a, uint32_t* __restrict__ oa, int blocks_a,
+__global__ void __launch_bounds__(128) order_scales_kernel(const uint8_t* __restrict__ sa, int64_t rows_a, uint32_t* __restrict__ oa, int blocks_a,
                                                           const uint8_t* __restrict__ sb, int64_t rows_b, uint32_t* __restrict__ ob, int64_t groups,
                                                           int kblocks, int fast) {
     pdl_launch_dependents();
@@ -278,11 +326,14 @@ __global__ void __launch_bounds__(128) tile_scales_kernel(const uint8_t* __restr
 }
 
 struct PairArgs {
+    const uint8_t *sa, *sb;   // scale bytes of A and B
     const uint16_t* bias;
     uint16_t* out;
     int64_t m, n;
     uint32_t idesc;
+    int64_t groups;
     int m_tiles, n_tiles, tiles, ksteps, tma_out;
+    int ordered;              // the scale bytes have been put in order ahead
 };
 
 template <bool FP4>
@@ -318,7 +369,7 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
     const int rank = (int)cluster_rank();
     const int first = (int)(blockIdx.x >> 1), step = (int)(gridDim.x >> 1);
     if (warp == 8 && lane == 0) {
-        for (int s = 0; s < S::kStages; ++s) { mbar_init(&full[s], rank == 0 ? 2 : 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(&full[s], (rank == 0 ? 2 : 1) + (a.ordered ? 0 : 8)); mbar_init(&empty[s], 1); }
         mbar_init(&acc_full, 1);
         mbar_init(&acc_empty, 16);
         mbar_init(&drained, 1);
@@ -348,11 +399,13 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
                 if (elect_one()) {
                     uint8_t* st = smem + sl.s * S::kStage;
                     uint64_t* bar = &full[sl.s];
-                    mbar_expect_tx(bar, 2 * S::kTile + S::kSfP + S::kSfQ);
+                    mbar_expect_tx(bar, 2 * S::kTile + (a.ordered ? S::kSfP + S::kSfQ : 0));
                     tma_load_2d(st, &map_a, j * 128, tm * 256 + rank * 128, bar);
                     tma_load_2d(st + S::kTile, &map_b, j * 128, tn * 256 + rank * 128, bar);
-                    tma_load_2d(st + S::kSfOff, &map_sa, j * (S::kBlk * 128), tm * 2 + rank, bar);
-                    tma_load_2d(st + S::kSfOff + S::kSfP, &map_sb, j * (S::kBlk * 128), tn * 2, bar);
+                    if (a.ordered) {
+                        tma_load_2d(st + S::kSfOff, &map_sa, j * (S::kBlk * 128), tm * 2 + rank, bar);
+                        tma_load_2d(st + S::kSfOff + S::kSfP, &map_sb, j * (S::kBlk * 128), tn * 2, bar);
+                    }
                 }
                 __syncwarp();
                 sl.advance();
@@ -414,6 +467,44 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
         const uint32_t acc = tmem + half * 128 + ((uint32_t)(warp & 3) << 21);
         const uint32_t empty0 = map_to_rank(smem_u32(&acc_empty), 0);
         uint8_t* os = smem + S::kOutOff + half * S::kOutBytes;
+        if (!a.ordered) {   // the pair's only tile: these warps have nothing to write yet
+            int tm, tn;
+            tile_place(first, a.m_tiles, a.n_tiles, tm, tn);
+            constexpr int W = kBatch * S::kBlk;
+            const int64_t row_p = (int64_t)tm * 256 + rank * 128 + t128, row_q = (int64_t)tn * 256 + threadIdx.x;
+            const uint32_t sf = smem_u32(smem) + S::kSfOff + (t128 & 31) * 16 + (t128 >> 5) * 4, sfq = sf + S::kSfP * (1 + half);
+            Slot<S::kStages> sl;
+            ScaleWords<W> p, q, next_p, next_q;
+            if (half == 0) p.load(a.sa, a.m, a.groups, row_p, 0);
+            q.load(a.sb, a.n, a.groups, row_q, 0);
+            for (int i = 0; i < a.ksteps && ok; i += kBatch) {
+                if (i + kBatch < a.ksteps) {
+                    const int64_t g = (int64_t)(i + kBatch) * (4 * S::kBlk);
+                    if (half == 0) next_p.load(a.sa, a.m, a.groups, row_p, g);
+                    next_q.load(a.sb, a.n, a.groups, row_q, g);
+                }
+                uint32_t wp[W], wq[W];
+                if (half == 0) p.place(wp);
+                q.place(wq);
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    if (i + u >= a.ksteps) break;
+                    ok = mbar_wait_warp(&empty[sl.s], sl.phase ^ 1);
+                    if (!ok) break;
+#pragma unroll
+                    for (int b = 0; b < S::kBlk; ++b) {
+                        if (half == 0) store_word(sf + sl.s * S::kStage + 512 * b, wp[u * S::kBlk + b]);
+                        store_word(sfq + sl.s * S::kStage + 512 * b, wq[u * S::kBlk + b]);
+                    }
+                    fence_async_shared();
+                    __syncwarp();
+                    if (elect_one()) mbar_arrive(&full[sl.s]);
+                    sl.advance();
+                }
+                p = next_p;
+                q = next_q;
+            }
+        }
         int it = 0;
         for (int t = first; t < a.tiles; t += step, ++it) {
             int tm, tn;
@@ -448,25 +539,29 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
             tc_fence_before();
             __syncwarp();
             if (elect_one()) mbar_arrive_peer(empty0);
+            const bool last = t + step >= a.tiles;   // the operands' shared memory is free: both 64 columns go out at once
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {   // 64 columns at a time
-                if (t128 == 0) bulk_wait_reads();
-                named_barrier(1 + half, 128);
+            for (int c = 0; c < 2; ++c) {
+                uint8_t* to = last && c == 1 ? smem + half * S::kOutBytes : os;
+                if (!(last && c == 1)) {
+                    if (t128 == 0) bulk_wait_reads();
+                    named_barrier(1 + half, 128);
+                }
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
-                    *reinterpret_cast<uint4*>(os + t128 * 128 + ((q ^ (t128 & 7)) << 4)) =
+                    *reinterpret_cast<uint4*>(to + t128 * 128 + ((q ^ (t128 & 7)) << 4)) =
                         make_uint4(w[32 * c + 4 * q], w[32 * c + 4 * q + 1], w[32 * c + 4 * q + 2], w[32 * c + 4 * q + 3]);
                 fence_async_shared();
                 named_barrier(1 + half, 128);
                 const int64_t nc = n0 + 64 * c;
                 if (a.tma_out) {
                     if (t128 == 0) {
-                        if (m0 < a.m && nc < a.n) tma_store_2d(&map_out, os, (int)nc, (int)m0);
+                        if (m0 < a.m && nc < a.n) tma_store_2d(&map_out, to, (int)nc, (int)m0);
                         bulk_commit();
                     }
                 } else {   // rows that do not start on 16 bytes: a warp writes one row at a time
                     for (int r = (warp & 3) * 32; r < (warp & 3) * 32 + 32 && m0 + r < a.m; ++r) {
-                        const uint32_t v = *reinterpret_cast<const uint32_t*>(os + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                        const uint32_t v = *reinterpret_cast<const uint32_t*>(to + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
                         uint16_t* o = a.out + (m0 + r) * a.n + nc + 2 * lane;
                         if (nc + 2 * lane < a.n) o[0] = (uint16_t)v;
                         if (nc + 2 * lane + 1 < a.n) o[1] = (uint16_t)(v >> 16);
@@ -485,16 +580,20 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
 // columns of scale blocks of a row of tiles, padded to whole steps of either format
 inline int64_t scale_blocks(int64_t k) { return ((k / 32 + 3) / 4 + 1) & ~int64_t(1); }
 
-// The scale bytes of both operands in tensor-core order, in the workspace, and the maps that load them: BLK blocks of one
-// row of tiles for A, of b_rows of them for B
-bool tile_scales(const MxMatmulArgs& x, int blk, int b_rows, CUtensorMap* map_a, CUtensorMap* map_b, cudaStream_t st) {
+// Pairs that take one tile each have warps to spare for fetching scale bytes; those that go on to further tiles have not,
+// and the kernel that puts the bytes in order first costs them little: 2 us of 1024 x 4096 x 4096 E4M3's 17.6, and a launch.
+inline bool orders_scales(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) > sm_count() / 2; }
+
+// The scale bytes of both operands in tensor-core order, in the workspace, and the maps that load them: blk blocks of 128
+// rows for A, of 256 for B
+bool order_scales(const MxMatmulArgs& x, int blk, CUtensorMap* map_a, CUtensorMap* map_b, cudaStream_t st) {
     const int64_t kb = scale_blocks(x.k), rb_a = (x.m + 127) / 128, rb_b = (x.n + 127) / 128, groups = x.k / 32;
     auto* sa = static_cast<uint32_t*>(x.workspace);
     uint32_t* sb = sa + rb_a * kb * 128;
-    if (!make_word_map(map_a, sa, rb_a, kb * 128, blk * 128, 1) || !make_word_map(map_b, sb, rb_b, kb * 128, blk * 128, b_rows)) return false;
+    if (!make_word_map(map_a, sa, rb_a, kb * 128, blk * 128, 1) || !make_word_map(map_b, sb, rb_b, kb * 128, blk * 128, 2)) return false;
     const int fast = groups % 16 == 0 && ((reinterpret_cast<uintptr_t>(x.a_scales) | reinterpret_cast<uintptr_t>(x.b_scales)) & 15) == 0;
     const dim3 grid((unsigned)(rb_a + rb_b), (unsigned)std::min<int64_t>((kb + 3) / 4, 64));
-    return launch_pdl(tile_scales_kernel, grid, dim3(128), 0, st, x.a_scales, x.m, sa, (int)rb_a, x.b_scales, x.n, sb, groups, (int)kb, fast) == cudaSuccess;
+    return launch_pdl(order_scales_kernel, grid, dim3(128), 0, st, x.a_scales, x.m, sa, (int)rb_a, x.b_scales, x.n, sb, groups, (int)kb, fast) == cudaSuccess;
 }
 
 template <bool FP4>
@@ -518,7 +617,11 @@ int go_pair(const MxMatmulArgs& x, cudaStream_t st) {
     if (!make_swizzled_map(&ma, x.a, x.m, row_bytes, row_bytes, 1, 128) || !make_swizzled_map(&mb, x.b, x.n, row_bytes, row_bytes, 1, 128)) return kErrLaunch;
     if (!a.tma_out) mo = ma;
     else if (!make_swizzled_map(&mo, x.out, x.m, x.n, x.n * 2, 2, 128)) return kErrLaunch;
-    if (!tile_scales(x, S::kBlk, 2, &msa, &msb, st)) return kErrLaunch;
+    a.sa = x.a_scales; a.sb = x.b_scales;
+    a.groups = x.k / 32;
+    a.ordered = orders_scales(x.m, x.n);
+    if (!a.ordered) msa = msb = ma;   // not used
+    else if (!order_scales(x, S::kBlk, &msa, &msb, st)) return kErrLaunch;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(2 * std::min(a.tiles, sm_count() / 2)));
     cfg.blockDim = dim3(320);
@@ -534,12 +637,8 @@ int go_pair(const MxMatmulArgs& x, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, kern, ma, mb, msa, msb, mo, a) == cudaSuccess ? check_launch() : kErrLaunch;
 }
 
-// Few tokens read the weights' scales once and in passing; more of them, and rows of scales that do not lie on four bytes,
-// are worth the kernel that puts the scales in order
-inline bool tiles_scales(int64_t m, int64_t k) { return m > 64 || k % 128 != 0; }
-
 template <bool FP4, int TN, bool SWAP>
-int go(const CUtensorMap& mp, const CUtensorMap& mq, const CUtensorMap& msp, const CUtensorMap& msq, const MmArgs& a, int64_t tiles, cudaStream_t st) {
+int go(const CUtensorMap& mp, const CUtensorMap& mq, const MmArgs& a, int64_t tiles, cudaStream_t st) {
     using S = MmShape<FP4, TN>;
     auto k = mx_matmul_kernel<FP4, TN, SWAP>;
     static SmemOptIn opt;
@@ -557,7 +656,7 @@ int go(const CUtensorMap& mp, const CUtensorMap& mq, const CUtensorMap& msp, con
     attr[1].val.clusterDim = {(unsigned)a.splits, 1, 1};
     cfg.attrs = attr;
     cfg.numAttrs = a.splits > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, k, mp, mq, msp, msq, a) == cudaSuccess ? check_launch() : kErrLaunch;
+    return cudaLaunchKernelEx(&cfg, k, mp, mq, a) == cudaSuccess ? check_launch() : kErrLaunch;
 }
 
 template <bool FP4>
@@ -581,26 +680,24 @@ int dispatch(const MxMatmulArgs& x, cudaStream_t st) {
     a.ktiles = (int)((row_bytes + 127) / 128);
     const int pf = swap ? x.b_fmt : x.a_fmt, qf = swap ? x.a_fmt : x.b_fmt;
     a.idesc = idesc_scaled(128, tn, FP4 ? 1u : (uint32_t)pf, FP4 ? 1u : (uint32_t)qf);
-    a.tiled_scales = tiles_scales(x.m, x.k);
     a.vec_out = x.n % 4 == 0 && (reinterpret_cast<uintptr_t>(x.out) & 7) == 0;   // eight bytes hold four columns
     const int64_t tiles = a.p_tiles * ((a.q_rows + tn - 1) / tn);
     a.splits = k_splits(tiles, a.ktiles, sm_count());
-    CUtensorMap mp, mq, msa, msb;
+    CUtensorMap mp, mq;
     if (!make_swizzled_map(&mp, p, a.p_rows, row_bytes, row_bytes, 1, kPRows)) return kErrLaunch;
     if (!make_swizzled_map(&mq, q, a.q_rows, row_bytes, row_bytes, 1, tn)) return kErrLaunch;
-    if (!a.tiled_scales) msa = msb = mp;   // not used
-    else if (!tile_scales(x, FP4 ? 2 : 1, 1, &msa, &msb, st)) return kErrLaunch;
-    const CUtensorMap &msp = swap ? msb : msa, &msq = swap ? msa : msb;
-    if (!swap) return go<FP4, 128, false>(mp, mq, msp, msq, a, tiles, st);
-    if (tn == 16) return go<FP4, 16, true>(mp, mq, msp, msq, a, tiles, st);
-    if (tn == 32) return go<FP4, 32, true>(mp, mq, msp, msq, a, tiles, st);
-    return go<FP4, 64, true>(mp, mq, msp, msq, a, tiles, st);
+    if (!swap) return go<FP4, 128, false>(mp, mq, a, tiles, st);
+    if (tn == 16) return go<FP4, 16, true>(mp, mq, a, tiles, st);
+    if (tn == 32) return go<FP4, 32, true>(mp, mq, a, tiles, st);
+    return go<FP4, 64, true>(mp, mq, a, tiles, st);
 }
 
 }  // namespace
 
-size_t mx_matmul_workspace(int64_t m, int64_t n, int64_t k) {
-    return tiles_scales(m, k) ? (size_t)(((m + 127) / 128 + (n + 127) / 128) * scale_blocks(k) * 512) : 0;
+size_t mx_matmul_workspace(int64_t m, int64_t n, int64_t k, int fp4) {
+    const int64_t steps = ((fp4 ? k / 2 : k) + 127) / 128;
+    if (m <= 64 || !takes_pairs(m, n, steps, sm_count()) || !orders_scales(m, n)) return 0;
+    return (size_t)(((m + 127) / 128 + (n + 127) / 128) * scale_blocks(k) * 512);
 }
 
 int launch_mx_matmul(const MxMatmulArgs& x, cudaStream_t st) {

@@ -410,8 +410,8 @@ at::Tensor mx_matmul(const at::Tensor& a, const at::Tensor& a_scales, const at::
     const bool fp8 = (a_format == MOR_B200_E4M3 || a_format == MOR_B200_E5M2) && (b_format == MOR_B200_E4M3 || b_format == MOR_B200_E5M2);
     TORCH_CHECK(fp4 || fp8, "mor::mx_matmul: formats must be 4 and 4 (E2M1), or each 0 (E4M3) or 1 (E5M2)");
     TORCH_CHECK(m >= 0 && n >= 0 && k > 0 && k % 32 == 0, "mor::mx_matmul: dim_k must be a positive multiple of 32");
-    at::Tensor ac = mx_payload(a, m, k, a_format, a, "mx_matmul", "a"), as = mx_part(a_scales, m, k / 32, a, 4, "mx_matmul", "a_scales");
-    at::Tensor bcod = mx_payload(b, n, k, b_format, a, "mx_matmul", "b"), bs = mx_part(b_scales, n, k / 32, a, 4, "mx_matmul", "b_scales");
+    at::Tensor ac = mx_payload(a, m, k, a_format, a, "mx_matmul", "a"), as = mx_part(a_scales, m, k / 32, a, 16, "mx_matmul", "a_scales");
+    at::Tensor bcod = mx_payload(b, n, k, b_format, a, "mx_matmul", "b"), bs = mx_part(b_scales, n, k / 32, a, 16, "mx_matmul", "b_scales");
     at::Tensor bi;
     if (bias.has_value() && bias->defined()) {
         TORCH_CHECK(bias->is_cuda() && bias->device() == a.device() && bias->scalar_type() == at::kBFloat16 && bias->dim() == 1 && bias->size(0) == n,
@@ -419,7 +419,7 @@ at::Tensor mx_matmul(const at::Tensor& a, const at::Tensor& a_scales, const at::
         bi = bias->contiguous();
     }
     at::Tensor out = mx_empty({m, n}, at::kBFloat16, a);
-    const size_t wsb = mor_b200_mx_matmul_workspace_bytes(m, n, k);
+    const size_t wsb = mor_b200_mx_matmul_workspace_bytes(m, n, k, (int)a_format);
     at::Tensor ws;
     if (wsb) ws = mx_empty({(int64_t)wsb}, at::kByte, a);
     check_status(mor_b200_mx_matmul(ac.data_ptr(), as.data_ptr(), bcod.data_ptr(), bs.data_ptr(), m, n, k, (int)a_format, (int)b_format,

@@ -263,7 +263,7 @@ def test_rows_beyond_the_result_are_left_alone():
         a, b, _ = product_case(m, n, 96, E4M3, E4M3, 4, False)
         args = [t.cuda() for t in (*a, *b)]
         out = torch.full((m * n + 4096,), 7.0, dtype=torch.bfloat16, device="cuda")
-        need = cabi.mx_lib().mor_b200_mx_matmul_workspace_bytes(m, n, 96)
+        need = cabi.mx_lib().mor_b200_mx_matmul_workspace_bytes(m, n, 96, 0)
         ws = torch.full((need + 64,), 5, dtype=torch.uint8, device="cuda")
         cabi.call("mor_b200_mx_matmul", *(t.data_ptr() for t in args), m, n, 96, 0, 0, None, out.data_ptr(), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
         assert bool((out[m * n:] == 7.0).all()) and bool((ws[need:] == 5).all())

@@ -82,8 +82,8 @@ def test_argument_errors_come_back_as_status_codes():
     assert m(p, p, p, p, 4, 4, 48, 0, 0, None, p, None, 0, None) == -2
     assert m(p + 8, p, p, p, 4, 4, 64, 0, 0, None, p, None, 0, None) == -2
     assert m(p, p, p + 8, p, 4, 4, 64, 0, 0, None, p, None, 0, None) == -2
-    assert m(p, p + 2, p, p, 4, 4, 64, 0, 0, None, p, None, 0, None) == -2
-    assert m(p, p, p, p + 1, 4, 4, 64, 0, 0, None, p, None, 0, None) == -2
+    assert m(p, p + 4, p, p, 4, 4, 64, 0, 0, None, p, None, 0, None) == -2
+    assert m(p, p, p, p + 8, 4, 4, 64, 0, 0, None, p, None, 0, None) == -2
     assert m(p, p, p, p, 4, 4, 64, 0, 0, p + 1, p, None, 0, None) == -2
     assert m(p, p, p, p, 4, 4, 64, 0, 0, None, p + 1, None, 0, None) == -2
     assert m(p, None, p, p, 4, 4, 64, 0, 0, None, p, None, 0, None) == -1
@@ -94,8 +94,9 @@ def test_argument_errors_come_back_as_status_codes():
     assert m(p, p, p, p, 4096, 4096, 64, 0, 0, None, p, p, 4096, None) == -3
     assert m(p, p, p, p, 4096, 4096, 64, 0, 0, None, p, p + 8, 1 << 20, None) == -3
     w = L.mor_b200_mx_matmul_workspace_bytes
-    assert w(4096, 4096, 64) == 64 * 2 * 512 and w(4097, 4096, 4096) == 65 * 32 * 512 and w(1, 4096, 4096) == 0 and w(1, 128, 32) == 2 * 2 * 512 and w(65, 128, 128) == 2 * 2 * 512
-    assert w(0, 1, 32) == 0 and w(4096, 4096, 48) == 0 and w(1 << 40, 1, 32) == 0
+    assert w(4096, 4096, 64, 0) == 64 * 2 * 512 and w(4097, 4096, 4096, 4) == 65 * 32 * 512
+    assert w(1, 4096, 4096, 4) == 0 and w(1, 128, 32, 0) == 0 and w(1024, 4096, 4096, 0) == 0   # one round of tiles
+    assert w(0, 1, 32, 0) == 0 and w(4096, 4096, 48, 0) == 0 and w(1 << 40, 1, 32, 0) == 0
     g = L.mor_b200_mx_matmul_grad
     assert g(p, 64, p, p, 4, 64, 64, 2, 0, p, None) == -1
     assert g(p, 64, p, p, 4, 64, 64, 0, 2, p, None) == -1
