@@ -7,8 +7,8 @@
 // The tensor core takes such a step of a 256 x 256 tile in 0.287 us (4.3 PFLOP/s 8-bit, 8.6 4-bit over 148 SMs), so a
 // kernel of this kind lives by handing it operands without a pause.  Measured: 8192^3 4-bit 190 us in a short run (5.8
 // PFLOP/s, tensor pipe 82 % active), 225 us in a long one, where the card's power limit lowers the clock; 8192 x 4096 x
-// 4096 E4M3 103 and 122 us (74 %).  Few tokens are bound by reading the weights: 24 x 16384 x 8192 E4M3 27 us (5.1 TB/s);
-// one token x 4096 x 4096 4-bit by latency, 5.4 us.
+// 4096 E4M3 103 and 122 us (74 %).  Few tokens are bound by reading the weights: 24 x 16384 x 8192 E4M3 28 us (5.0 TB/s);
+// one token x 4096 x 4096 4-bit by latency, 5.8 us.
 #include <algorithm>
 
 #include "mx_kernels.cuh"
@@ -581,7 +581,8 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
 inline int64_t scale_blocks(int64_t k) { return ((k / 32 + 3) / 4 + 1) & ~int64_t(1); }
 
 // Pairs that take one tile each have warps to spare for fetching scale bytes; those that go on to further tiles have not,
-// and the kernel that puts the bytes in order first costs them little: 2 us of 1024 x 4096 x 4096 E4M3's 17.6, and a launch.
+// and the kernel that puts the bytes in order first costs them little.  It costs the others a launch and about a microsecond:
+// 1024 x 4096 x 4096 E4M3 17.6 us with it, 16.8 without.
 inline bool orders_scales(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) > sm_count() / 2; }
 
 // The scale bytes of both operands in tensor-core order, in the workspace, and the maps that load them: blk blocks of 128

@@ -262,11 +262,13 @@ inline int k_splits(int64_t tiles, int64_t steps, int sms) {
 }
 // Pairs of CTAs on 256 x 256 or single ones on 128 x 128?  A pair takes a step in about the time of a single CTA with four
 // times the result, so pairs win unless few tiles let single CTAs split the sum: each step saved is worth about 0.3 us,
-// meeting in the cluster costs about 4.  Measured on both sides: 128 x 4096 x 4096 E4M3 (32 steps, four splits) 15.5 us in pairs, 12.6 single;
-// 4-bit (16 steps) 11.0 and 11.3; 512 x 1024 x 8192 E4M3 24.1 and 15.0; 1024^3 8.3 and 9.9; 1536 x 1536 x 4096 16.3 and 20.6.
+// meeting in the cluster costs about 3.  Measured on both sides, pairs and single, in us (steps saved): 128 x 4096 x 4096
+// E4M3 15.6 and 12.1 (24), 4-bit 11.6 and 11.0 (12); 256 x 4096 x 4096 E4M3 15.7 and 14.0 (16), 4-bit 11.7 and 12.0 (8);
+// 512 x 1024 x 8192 E4M3 25.5 and 14.9 (48); 1111 x 1003 x 2080 4-bit 11.7 and 12.6 (5); 1536 x 1536 x 4096 E4M3 16.1 and
+// 20.1 (0); gradients 128 x 4096 x 4096 27.2 and 17.0 (48), 1024^3 10.9 and 12.3 (8).
 inline bool takes_pairs(int64_t m, int64_t n, int64_t steps, int sms) {
     const int s = k_splits(((m + 127) / 128) * ((n + 127) / 128), steps, sms);
-    return steps - steps / s < 14;
+    return steps - steps / s < 12;
 }
 
 // row-major matrix of bytes (or bf16) with a row pitch, boxes of 128 bytes x box_rows under the 128-byte swizzle; what lies outside reads as zero

@@ -515,6 +515,24 @@ at::Tensor mx_linear(const at::Tensor& x, const at::Tensor& weight, const std::o
     return MxLinear::apply(x, weight, bias, format);
 }
 
+// The forward pass alone, from weights that were quantised once.
+at::Tensor mx_linear_packed(const at::Tensor& x, const at::Tensor& payload, const at::Tensor& scales, const std::optional<at::Tensor>& bias,
+                            int64_t format) {
+    TORCH_CHECK(x.is_cuda(), "mor::mx_linear_packed: x must be a CUDA tensor");
+    TORCH_CHECK(format == MOR_B200_E4M3 || format == MOR_B200_E5M2 || format == MOR_B200_MX_E2M1,
+                "mor::mx_linear_packed: elem_format must be 0 (E4M3), 1 (E5M2) or 4 (E2M1)");
+    TORCH_CHECK(payload.dim() == 2 && x.dim() >= 1, "mor::mx_linear_packed: x must be [..., in] and payload that of [out, in]");
+    const at::NoGradGuard none;
+    const int64_t k = x.size(-1), n = payload.size(0);
+    at::Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, k});
+    const std::vector<at::Tensor> q = mx_quantized(x2, format);
+    at::Tensor y = mx_matmul(q[0], q[1], payload, scales, x2.size(0), n, k, format, format, bias);
+    if (x.dim() == 2) return y;
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = n;
+    return y.reshape(shape);
+}
+
 }  // namespace
 
 // Registers _C as a Python extension module.
@@ -549,6 +567,7 @@ TORCH_LIBRARY(mor, m) {
   m.def("mx_matmul(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, int dim_m, int dim_n, int dim_k, int a_format, int b_format, Tensor? bias) -> Tensor");
   m.def("mx_matmul_grad(Tensor g, Tensor payload, Tensor scales, int dim_m, int dim_n, int dim_k, int elem_format, bool transpose_g) -> Tensor");
   m.def("mx_linear(Tensor x, Tensor weight, Tensor? bias, int elem_format) -> Tensor", &mx_linear);   // composed of the above, with its gradient
+  m.def("mx_linear_packed(Tensor x, Tensor payload, Tensor scales, Tensor? bias, int elem_format) -> Tensor", &mx_linear_packed);
 }
 
 TORCH_LIBRARY_IMPL(mor, CUDA, m) {

@@ -253,10 +253,5 @@ class PackedMXLinear(torch.nn.Module):
         self.register_buffer("scales", scales.contiguous())
         self.register_buffer("bias", None if layer.bias is None else layer.bias.detach().to(torch.bfloat16, copy=True))
 
-    @torch.no_grad()
     def forward(self, x: Tensor) -> Tensor:
-        f = MX_FORMATS[self.elem_format]
-        x2 = x.reshape(-1, x.shape[-1])
-        xc, xs = _mx_quantize(x2, f)
-        y = ops.mx_matmul(xc, xs, self.payload, self.scales, x2.shape[0], self.out_features, self.in_features, f, f, self.bias)
-        return y.reshape(*x.shape[:-1], self.out_features)
+        return torch.ops.mor.mx_linear_packed.default(x, self.payload, self.scales, self.bias, MX_FORMATS[self.elem_format])

@@ -128,7 +128,11 @@ def test_what_is_kept_is_the_codes(name):
 def test_packed_layer_gives_the_same_bits(name, tokens):
     layer, x, _ = make(name, (tokens, 512), 1000)
     packed = layer.pack()
-    assert torch.equal(packed(x), layer(x).detach())
+    y = packed(x)
+    assert torch.equal(y, layer(x).detach()) and not y.requires_grad
+    assert torch.equal(packed(x[None, :, None]), y[None, :, None])
+    with pytest.raises(RuntimeError, match="must be"):
+        packed(x[:, :64])
     assert not list(packed.parameters()) and "payload" in packed.state_dict()
     with torch.no_grad():
         layer.weight.zero_()
