@@ -104,6 +104,7 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
     extern __shared__ uint8_t s_raw[];
     __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], acc_done, drained;
     __shared__ uint32_t s_tmem;
+    __shared__ int s_late;   // a wait ran out: copies may still land where the result would pass through
     uint8_t* smem = s_raw + ((1024 - (smem_u32(s_raw) & 1023)) & 1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -117,6 +118,7 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
         for (int s = 0; s < S::kStages; ++s) { mbar_init(&full[s], 1 + 4); mbar_init(&empty[s], 1); }
         mbar_init(&acc_done, 1);
         mbar_init(&drained, 1);
+        s_late = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_p));
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q));
     }
@@ -214,6 +216,7 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
             q = next_q;
         }
         ok = ok && mbar_wait_warp(&acc_done, 0);
+        if (!ok) s_late = 1;
         tc_fence_after();
     }
 
@@ -246,6 +249,7 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
     else if (warp < 4) named_barrier(1, 128);
     if (warp < 4) {
         const int rows = sums.rows(), first_row = split * rows;
+        const float late = s_late ? u2f(0x7FFFFFFFu) : 0.0f;
         if constexpr (SWAP) {
             // out's rows run along P: a lane takes one P row, a warp four tokens at a time
             for (int i = threadIdx.x; i < rows * (TN / 4); i += 128) {
@@ -253,7 +257,7 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
                 const int64_t p = p0 + first_row + r;
                 if (p >= a.p_rows || q0 + c >= a.q_rows) continue;
                 const float4 v = sums.sum4(r, c);
-                const float bias = a.bias ? u2f((uint32_t)__ldg(a.bias + p) << 16) : 0.0f;
+                const float bias = (a.bias ? u2f((uint32_t)__ldg(a.bias + p) << 16) : 0.0f) + late;
                 const float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -263,11 +267,11 @@ __global__ void __launch_bounds__(192, 1) mx_matmul_kernel(const __grid_constant
             constexpr int kLanes = TN / 4;   // a lane takes four columns
             const int c = (threadIdx.x % kLanes) * 4;
             const int64_t q = q0 + c;
-            float bias[4] = {};
+            float bias[4] = {late, late, late, late};
             if (a.bias)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (q + j < a.q_rows) bias[j] = u2f((uint32_t)__ldg(a.bias + q + j) << 16);
+                    if (q + j < a.q_rows) bias[j] += u2f((uint32_t)__ldg(a.bias + q + j) << 16);
 #pragma unroll 4
             for (int r = threadIdx.x / kLanes; r < rows; r += 128 / kLanes) {
                 const int64_t p = p0 + first_row + r;
@@ -364,6 +368,7 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
     __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], acc_full, acc_empty, drained;
     __shared__ uint32_t s_tmem;
     __shared__ __align__(16) float s_bias[256];
+    __shared__ int s_late[2];   // a wait ran out: copies may still land in the operands' memory
     uint8_t* smem = s_raw + ((1024 - (smem_u32(s_raw) & 1023)) & 1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
@@ -373,6 +378,7 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
         mbar_init(&acc_full, 1);
         mbar_init(&acc_empty, 16);
         mbar_init(&drained, 1);
+        s_late[0] = s_late[1] = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a));
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b));
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_sa));
@@ -534,23 +540,28 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
                     }
                 }
 #pragma unroll
-                for (int e = 0; e < 16; ++e) w[16 * c + e] = ok ? pack_bf16_rne(u2f(r[2 * e + 1]), u2f(r[2 * e])) : 0x7FFF7FFFu;
+                for (int e = 0; e < 16; ++e) w[16 * c + e] = pack_bf16_rne(u2f(r[2 * e + 1]), u2f(r[2 * e]));
             }
             tc_fence_before();
             __syncwarp();
             if (elect_one()) mbar_arrive_peer(empty0);
-            const bool last = t + step >= a.tiles;   // the operands' shared memory is free: both 64 columns go out at once
+            if (!ok) s_late[half] = 1;
+            bool at_once = false;   // after the last tile the operands' shared memory is free: both 64 columns go out at once
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                uint8_t* to = last && c == 1 ? smem + half * S::kOutBytes : os;
-                if (!(last && c == 1)) {
+                uint8_t* to = c == 1 && at_once ? smem + half * S::kOutBytes : os;
+                if (c == 0 || !at_once) {
                     if (t128 == 0) bulk_wait_reads();
                     named_barrier(1 + half, 128);
                 }
+                const bool late = s_late[half] != 0;
+                if (c == 0) at_once = !late && t + step >= a.tiles;
 #pragma unroll
-                for (int q = 0; q < 8; ++q)
+                for (int q = 0; q < 8; ++q) {
+                    const uint32_t* v = w + 32 * c + 4 * q;
                     *reinterpret_cast<uint4*>(to + t128 * 128 + ((q ^ (t128 & 7)) << 4)) =
-                        make_uint4(w[32 * c + 4 * q], w[32 * c + 4 * q + 1], w[32 * c + 4 * q + 2], w[32 * c + 4 * q + 3]);
+                        late ? make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu) : make_uint4(v[0], v[1], v[2], v[3]);
+                }
                 fence_async_shared();
                 named_barrier(1 + half, 128);
                 const int64_t nc = n0 + 64 * c;
