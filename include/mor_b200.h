@@ -187,7 +187,7 @@ MOR_B200_API int mor_b200_block_scaling_delayed_t(const void* input, void* outpu
  * aligned -- the fp8 code for E4M3 (format 0) / E5M2 (1), the 6-bit code in a byte for E2M3 (3).
  * scales: one E8M0 byte per 1 x block_cols group [rows, cols / block_cols], MX convention:
  * element = decode(code) * 2^(scale - 127); an all-zero group gets 127.  block_cols a power of
- * two from 8 to 256, rows * cols a multiple of 256.  decode * scale equals the fake-quantized
+ * two from 8 to 256.  decode * scale equals the fake-quantized
  * output bit for bit, except where the code is zero under a scale below one (fake quantization
  * returns 2^(-e8-127) there, an artefact of its exponent-field arithmetic, :296-305). */
 MOR_B200_API int mor_b200_quantize_mx(const void* input, void* payload, void* scales, int64_t rows, int64_t cols,

@@ -347,10 +347,13 @@ mx_quantize_kernel(const uint4* __restrict__ in, uint2* __restrict__ payload, ui
             }
         } else {  // last, partial chunk, or a copy that did not arrive: ordinary loads
             for (int r = 0; r * 32 < nv; ++r) {
+                const bool inside = r * 32 + lane < nv;   // whole groups: a row is a multiple of them
                 uint32_t sb;
-                const uint2 codes = mx_codes_one<FMT, GS>(ld_stream(in + v0 + r * 32 + lane), sb);
-                store_codes<PACK6>(payload, o + r * 32, codes);
-                if (scale_lane) sc[r * (32 >> GS)] = (uint8_t)sb;
+                const uint2 codes = mx_codes_one<FMT, GS>(inside ? ld_stream(in + v0 + r * 32 + lane) : make_uint4(0u, 0u, 0u, 0u), sb);
+                if (inside) {
+                    store_codes<PACK6>(payload, o + r * 32, codes);
+                    if (scale_lane) sc[r * (32 >> GS)] = (uint8_t)sb;
+                }
             }
         }
         ws.release(st, c + kMxStages * n_warps);
@@ -538,7 +541,7 @@ int launch_quantize_mx(const void* in, void* payload, uint8_t* scales, int64_t r
     if (bcols % 8 || cols % bcols) return kErrUnsupportedShape;
     const int gvec = bcols / 8;
     const int64_t nvec = rows * cols / 8;
-    if (gvec > 32 || (gvec & (gvec - 1)) || nvec % 32) return kErrUnsupportedShape;
+    if (gvec > 32 || (gvec & (gvec - 1))) return kErrUnsupportedShape;
     int shift = 0;
     while ((1 << shift) < gvec) ++shift;
     constexpr int kRing = kMxWarps * kMxStages * kMxChunkVec * 16;

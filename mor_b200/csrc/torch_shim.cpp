@@ -450,16 +450,16 @@ at::Tensor mx_matmul_grad(const at::Tensor& g, const at::Tensor& payload, const 
 }
 
 // ---- a linear layer on microscaled operands -----------------------------------------------
-// Codes and scale bytes of a [rows, cols] tensor in groups of 32 columns; quantize_mx takes whole multiples of 256 elements.
+// Codes and scale bytes of a [rows, cols] tensor in groups of 32 columns.
 std::vector<at::Tensor> mx_quantized(const at::Tensor& x, int64_t format) {
     const int64_t r = x.size(0), c = x.size(1);
     if (format == MOR_B200_MX_E2M1) return quantize_mx_fp4(x, r, c, 32);
-    int64_t rows = 256;
-    for (int64_t d = c; rows > 1 && d % 2 == 0; d /= 2) rows /= 2;   // 256 / gcd(c, 256)
-    const int64_t padded = std::max((r + rows - 1) / rows, int64_t(1)) * rows;
-    if (padded == r) return quantize_mx(x, r, c, 32, format);
-    std::vector<at::Tensor> q = quantize_mx(at::constant_pad_nd(x, {0, 0, 0, padded - r}), padded, c, 32, format);
-    return {q[0].narrow(0, 0, r), q[1].narrow(0, 0, r)};
+    TORCH_CHECK(x.scalar_type() == at::kBFloat16 && c > 0 && c % 32 == 0,
+                "mor::mx_linear: 8-bit operands are quantised from bfloat16, with a width that is a positive multiple of 32");
+    if (r == 0) return {mx_empty({0, c}, at::kByte, x), mx_empty({0, c / 32}, at::kByte, x)};
+    at::Tensor packed = x.contiguous();
+    if (reinterpret_cast<uintptr_t>(packed.data_ptr()) % 16) packed = packed.clone();
+    return quantize_mx(packed, r, c, 32, format);
 }
 
 // Straight-through: the gradients are those of a linear layer fed the quantised values, computed from the codes, which are

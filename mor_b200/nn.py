@@ -17,7 +17,6 @@ ordinary tensor operations and is a logging aid, not part of the bit-exact path.
 """
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 from typing import Callable, List, Optional
 
@@ -193,14 +192,7 @@ MX_FORMATS = {"e4m3": 0, "e5m2": 1, "e2m1": 4}
 def _mx_quantize(x: Tensor, elem_format: int):
     """Codes and scale bytes of a ``[rows, cols]`` tensor in groups of 32 columns."""
     r, c = x.shape
-    if elem_format == 4:
-        return ops.quantize_mx_fp4(x, r, c, 32)
-    whole = 256 // math.gcd(c, 256)             # quantize_mx takes whole multiples of 256 elements
-    padded = max(-(-r // whole), 1) * whole
-    if padded == r:
-        return ops.quantize_mx(x, r, c, 32, elem_format)
-    codes, scales = ops.quantize_mx(torch.nn.functional.pad(x, (0, 0, 0, padded - r)), padded, c, 32, elem_format)
-    return codes[:r], scales[:r]
+    return ops.quantize_mx_fp4(x, r, c, 32) if elem_format == 4 else ops.quantize_mx(x, r, c, 32, elem_format)
 
 
 def mx_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, elem_format: int = 0) -> Tensor:

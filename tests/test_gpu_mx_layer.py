@@ -102,6 +102,26 @@ def test_float32_layer_and_partial_gradients():
     assert torch.isfinite(layer.weight.grad).all()
 
 
+@pytest.mark.parametrize("fmt", [0, 1, 3])
+@pytest.mark.parametrize("rows,cols,by", [(1, 32, 32), (3, 32, 32), (1, 8, 8), (5, 96, 32), (129, 32, 16), (141, 64, 64), (67, 4128, 32), (1000, 40, 8)])
+def test_eight_bit_quantisation_of_any_number_of_rows(rows, cols, by, fmt):
+    """sizes that are no multiple of 256 elements, against the CPU oracle, and nothing written behind them"""
+    import oracle
+    from mor_b200 import cabi
+    x = torch.randn(rows, cols, generator=torch.Generator().manual_seed(rows)).to(torch.bfloat16)
+    codes, scales = oracle.quantize_mx(oracle.bf16_bits(x), by, fmt)
+    d = x.cuda()
+    p = torch.full((rows * cols + 512,), 9, dtype=torch.uint8, device="cuda")
+    s = torch.full((rows * cols // by + 512,), 9, dtype=torch.uint8, device="cuda")
+    cabi.call("mor_b200_quantize_mx", d.data_ptr(), p.data_ptr(), s.data_ptr(), rows, cols, by, fmt, torch.cuda.current_stream().cuda_stream)
+    assert (p[:rows * cols].cpu().numpy() == codes.reshape(-1)).all() and (s[:rows * cols // by].cpu().numpy() == scales.reshape(-1)).all()
+    assert bool((p[rows * cols:] == 9).all()) and bool((s[rows * cols // by:] == 9).all())
+    if fmt == 3:
+        p6 = torch.full((rows * cols * 3 // 4 + 512,), 9, dtype=torch.uint8, device="cuda")
+        cabi.call("mor_b200_quantize_mx_fp6", d.data_ptr(), p6.data_ptr(), s.data_ptr(), rows, cols, by, torch.cuda.current_stream().cuda_stream)
+        assert (p6[:rows * cols * 3 // 4].cpu().numpy() == oracle.pack_fp6(codes).reshape(-1)).all() and bool((p6[rows * cols * 3 // 4:] == 9).all())
+
+
 @pytest.mark.parametrize("name", ["e4m3", "e2m1"])
 def test_no_tokens(name):
     layer, x, g = make(name, (0, 64), 40)
