@@ -16,6 +16,7 @@
 // active), 213 to 224 us in a long one (power limit).  One widening group of eight warps takes 27 % longer than two, three
 // groups of four are best: what counts is that a group's waits hide behind the others' work.
 #include <algorithm>
+#include <type_traits>
 
 #include "mx_kernels.cuh"
 #include "tcgen05.cuh"
@@ -29,6 +30,7 @@ struct GrArgs {
     int64_t m, n, k, groups;
     int m_tiles, n_tiles, tiles;
     int ksteps, across, splits, fast_scales;
+    PairWork work;              // pairs
 };
 
 constexpr int kTK = 64;                 // k a step: 128 bytes of bf16
@@ -140,6 +142,14 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
     const int step = CG == 2 ? (int)(gridDim.x >> 1) : (int)(gridDim.x / (unsigned)a.splits);
     const int k_first = (int)((int64_t)a.ksteps * split / a.splits), k_last = (int)((int64_t)a.ksteps * (split + 1) / a.splits);
     const int ks = k_last - k_first;
+    // piece by piece: a tile, and which half of its columns
+    auto piece = [&](int i, int& tile, int& half) {
+        if constexpr (CG == 2) return a.work.piece(i, first, tile, half);
+        tile = first + i * step;
+        half = -1;
+        return tile < a.tiles;
+    };
+    const int64_t whole = CG == 2 ? (a.work.halves ? (int64_t)a.work.rounds * ks : INT64_MAX) : INT64_MAX;   // steps before those of a half tile
 
     if (warp == 4 && lane == 0) {
         for (int s = 0; s < S::kSA; ++s) { mbar_init(&full_a[s], 1); mbar_init(&empty_a[s], 1); }
@@ -166,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
     const ClusterSum<S::kTN> sums{smem_u32(smem), a.splits, split};
     if (warp == 4) {
         Slot<S::kSA> sa;
-        for (int t = first; t < a.tiles && ok; t += step) {
+        for (int i = 0, t, half; ok && piece(i, t, half); ++i) {
             int tm, tn;
             tile_place(t, a.m_tiles, a.n_tiles, tm, tn);
             const int m0 = tm * S::kTM + rank * 128;
@@ -192,16 +202,16 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
             for (int s = 0; s < S::kSA; ++s) mbar_wait_bounded(&full_a[s], s < sa.s ? sa.phase : sa.phase ^ 1);
     } else if (warp == 5) {
         if (rank == 0) {
-            const uint32_t idesc = idesc_bf16(S::kTM, S::kTN, a.across != 0, true);
+            const uint32_t idesc_whole = idesc_bf16(S::kTM, S::kTN, a.across != 0, true), idesc_half = idesc_bf16(S::kTM, S::kTN / 2, a.across != 0, true);
             const uint32_t step_a = a.across ? 2048 / 16 : 32 / 16;
             // operands whose rows run along m (n): 64 of them to a 128-byte row, such columns of tiles 8 KiB apart, eight k 1 KiB
             const uint64_t da0 = a.across ? umma_desc(smem_u32(smem), 8192, 1024, kLayoutSwizzle128) : umma_desc_kmajor(smem_u32(smem));
             const uint64_t db0 = umma_desc(smem_u32(smem + S::kBOff), 8192, 1024, kLayoutSwizzle128);
             Slot<S::kSA> sa;
             Slot<S::kSB> sb;
-            int it = 0;
-            for (int t = first; t < a.tiles && ok; t += step, ++it) {
+            for (int it = 0, t, half; ok && piece(it, t, half); ++it) {
                 const int b = it & 1;
+                const uint32_t idesc = half < 0 ? idesc_whole : idesc_half;
                 if (it >= 2) ok = mbar_wait_cluster(&acc_empty[b], (it / 2 - 1) & 1);
                 if (!ok) break;
                 for (int j = 0; j < ks; ++j) {
@@ -230,10 +240,11 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
         }
     } else if (warp == 6) {
         Slot<S::kSC> sc;
-        for (int t = first; t < a.tiles && ok; t += step) {
+        for (int i = 0, t, half; ok && piece(i, t, half); ++i) {
             int tm, tn;
             tile_place(t, a.m_tiles, a.n_tiles, tm, tn);
-            const int n0 = tn * S::kTN + rank * NB;
+            // of a half tile each CTA widens 64 columns; the copy brings 64 more, which nobody reads
+            const int n0 = tn * S::kTN + (half < 0 ? rank * NB : half * NB + rank * (NB / 2));
             for (int j = 0; j < ks; ++j) {
                 ok = mbar_wait_warp(&empty_c[sc.s], sc.phase ^ 1);
                 if (!ok) break;
@@ -253,10 +264,10 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
         const uint32_t dst0 = smem_u32(smem + S::kCOff + S::kCodeBytes) + 4 * r;
         const int64_t stride = (int64_t)kTK * a.groups;
         Slot<S::kSC> sc;
-        for (int t = first; t < a.tiles && ok; t += step) {
+        for (int i = 0, t, half; ok && piece(i, t, half); ++i) {
             int tm, tn;
             tile_place(t, a.m_tiles, a.n_tiles, tm, tn);
-            const int grp = (tn * S::kTN + rank * NB) / 32;
+            const int grp = (tn * S::kTN + (half < 0 ? rank : half) * NB) / 32;   // both CTAs of a half tile share four groups
             int64_t left = grp < a.groups ? a.k - (int64_t)k_first * kTK - r : 0;   // this lane's k is inside while positive
             const uint8_t* src = a.scales + ((int64_t)k_first * kTK + r) * a.groups + grp;
             for (int j = 0; j < ks; ++j) {
@@ -287,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
         const int ct = (threadIdx.x - 32 * kFirstConv) % (32 * kConvWarps), group = (warp - kFirstConv) / kConvWarps, u = ct & 7, nc = (ct / 8) % (NB / 64), r0 = ct / kLanesPerRow;
         const uint32_t wide0 = CG == 2 ? map_to_rank(smem_u32(&wide[0]), 0) : smem_u32(&wide[0]);   // the pair's issuer waits for both halves
         const int sbyte = nc * 2 + (u >> 2);
-        const int64_t total = first < a.tiles ? (int64_t)((a.tiles - 1 - first) / step + 1) * ks : 0;
+        const int64_t total = CG == 2 ? (int64_t)a.work.pieces(first) * ks : (first < a.tiles ? (int64_t)((a.tiles - 1 - first) / step + 1) * ks : 0);
         Slot<S::kSA> sa;
         Slot<S::kSB> sb;
         Slot<S::kSC> sc;
@@ -296,27 +307,37 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
             ok = mbar_wait_warp(&full_c[sc.s], sc.phase);
             if (!ok) break;
             const uint8_t* cs = smem + S::kCOff + sc.s * S::kCStage;
-            uint2 c[kPasses];
-            uint32_t k8[kPasses], odd = 0;
+            uint8_t* bs = smem + S::kBOff + sb.s * S::kBBytes;
+            // rows r, r + ROWS, ... of eight columns each; passes are a multiple of eight rows apart: the same swizzle
+            auto widen = [&](auto passes, int rows, int r, int col, int scale_byte, uint8_t* to) {
+                constexpr int P = decltype(passes)::value;
+                uint2 c[P];
+                uint32_t k8[P], odd = 0;
 #pragma unroll
-            for (int p = 0; p < kPasses; ++p) {
-                const int row = r0 + p * kRowsPerPass;
-                if constexpr (FMT == kE2M1) c[p] = make_uint2(*reinterpret_cast<const uint32_t*>(cs + row * S::kRowBytes + nc * 32 + u * 4), 0u);
-                else c[p] = *reinterpret_cast<const uint2*>(cs + row * S::kRowBytes + nc * 64 + u * 8);
-                k8[p] = cs[S::kCodeBytes + 4 * row + sbyte];
+                for (int p = 0; p < P; ++p) {
+                    const int row = r + p * rows;
+                    if constexpr (FMT == kE2M1) c[p] = make_uint2(*reinterpret_cast<const uint32_t*>(cs + row * S::kRowBytes + col / 2), 0u);
+                    else c[p] = *reinterpret_cast<const uint2*>(cs + row * S::kRowBytes + col);
+                    k8[p] = cs[S::kCodeBytes + 4 * row + scale_byte];
+                }
+                __syncwarp();
+                if (elect_one()) mbar_arrive(&empty_c[sc.s]);
+                if (!mbar_wait_warp(&empty_b[sb.s], sb.phase ^ 1)) return false;
+#pragma unroll
+                for (int p = 0; p < P; ++p) *reinterpret_cast<uint4*>(to + p * rows * 128) = widen8<FMT>(c[p], k8[p], odd);
+                if (odd & kOdd) {
+#pragma unroll
+                    for (int p = 0; p < P; ++p) *reinterpret_cast<uint4*>(to + p * rows * 128) = widen8_any<FMT>(c[p], k8[p]);
+                }
+                return true;
+            };
+            if (i < whole) {
+                ok = widen(std::integral_constant<int, kPasses>{}, kRowsPerPass, r0, nc * 64 + u * 8, sbyte, bs + nc * 8192 + r0 * 128 + ((u ^ (r0 & 7)) << 4));
+            } else {   // 64 columns: all lanes on them
+                const int r = ct >> 3;
+                ok = widen(std::integral_constant<int, kPasses / 2>{}, 2 * kRowsPerPass, r, u * 8, rank * 2 + (u >> 2), bs + r * 128 + ((u ^ (r & 7)) << 4));
             }
-            __syncwarp();
-            if (elect_one()) mbar_arrive(&empty_c[sc.s]);
-            ok = mbar_wait_warp(&empty_b[sb.s], sb.phase ^ 1);
             if (!ok) break;
-            uint8_t* bs = smem + S::kBOff + sb.s * S::kBBytes + nc * 8192 + r0 * 128 + ((u ^ (r0 & 7)) << 4);
-#pragma unroll
-            for (int p = 0; p < kPasses; ++p)   // passes are a multiple of eight rows apart: the same swizzle
-                *reinterpret_cast<uint4*>(bs + p * (kRowsPerPass * 128)) = widen8<FMT>(c[p], k8[p], odd);
-            if (odd & kOdd) {
-#pragma unroll
-                for (int p = 0; p < kPasses; ++p) *reinterpret_cast<uint4*>(bs + p * (kRowsPerPass * 128)) = widen8_any<FMT>(c[p], k8[p]);
-            }
             fence_async_shared();
             if (ct < 32) ok = mbar_wait_warp(&full_a[sa.s], sa.phase);   // one warp's arrival vouches for the gradient's tile
             if (!ok) break;
@@ -328,14 +349,13 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
         }
         static_assert(kRowsPerPass % 8 == 0 && kConvGroups <= S::kSA && kConvGroups <= S::kSB && kConvGroups <= S::kSC, "swizzle, first slots");
     } else {
-        int it = 0;
         const uint32_t sums_to = sums.place(threadIdx.x);
         const uint32_t empty0 = CG == 2 ? map_to_rank(smem_u32(&acc_empty[0]), 0) : smem_u32(&acc_empty[0]);
         int ob = 0;
-        for (int t = first; t < a.tiles; t += step, ++it) {
+        for (int it = 0, t, half; piece(it, t, half); ++it) {
             int tm, tn;
             tile_place(t, a.m_tiles, a.n_tiles, tm, tn);
-            const int m0 = tm * S::kTM + rank * 128, n0 = tn * S::kTN;
+            const int m0 = tm * S::kTM + rank * 128, n0 = tn * S::kTN + (half > 0 ? NB : 0), columns = half < 0 ? S::kTN : S::kTN / 2;
             const int b = it & 1;
             ok = ok && mbar_wait_warp(&acc_full[b], (it / 2) & 1);
             if (!ok) s_late = 1;
@@ -343,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
             const uint32_t acc = tmem + b * S::kTN + ((uint32_t)warp << 21);
             if (CG == 1 && a.splits > 1) cluster_sync();   // no CTA is still reading operands; the other warps meet this below
 #pragma unroll 1
-            for (int c0 = 0; c0 < S::kTN; c0 += 64) {
+            for (int c0 = 0; c0 < columns; c0 += 64) {
                 uint32_t r[2][32];
                 tmem_load32(acc + c0, r[0]);
                 tmem_load32(acc + c0 + 32, r[1]);
@@ -443,7 +463,8 @@ int go(const MxGradArgs& x, cudaStream_t st) {
     a.splits = 1;
     int grid;
     if constexpr (CG == 2) {
-        grid = 2 * std::min(a.tiles, sm_count() / 2);
+        a.work = pair_work(a.tiles, sm_count());
+        grid = 2 * a.work.launched();
     } else {
         a.splits = k_splits(a.tiles, a.ksteps, sm_count());
         grid = a.splits > 1 ? a.tiles * a.splits : std::min(a.tiles, sm_count());

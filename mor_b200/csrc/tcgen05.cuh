@@ -253,6 +253,34 @@ __device__ __forceinline__ void tile_place(int t, int m_tiles, int n_tiles, int&
     tm = band * kBand + in - tn * rows;
 }
 
+// The work of the pairs of CTAs on 256 x 256 tiles: `rounds` whole tiles each, then the tiles that are left, as halves of 128
+// columns where there are pairs for them: a last round of few tiles then takes a little over half as long.
+struct PairWork {
+    int pairs, rounds, rest, halves;
+    __host__ __device__ int launched() const { return rounds ? pairs : (halves ? 2 * rest : rest); }
+    // the i-th piece of a pair: a tile, and which half of its columns (-1: all)
+    __device__ __forceinline__ bool piece(int i, int pair, int& tile, int& half) const {
+        half = -1;
+        tile = i * pairs + pair;
+        if (i < rounds) return true;
+        if (i > rounds || pair >= (halves ? 2 * rest : rest)) return false;
+        if (halves) {
+            half = pair & 1;
+            tile = rounds * pairs + (pair >> 1);
+        }
+        return true;
+    }
+    __device__ __forceinline__ int pieces(int pair) const { return rounds + (pair < (halves ? 2 * rest : rest) ? 1 : 0); }
+};
+inline PairWork pair_work(int64_t tiles, int sms) {
+    PairWork w = {};
+    w.pairs = sms / 2;
+    w.rounds = (int)(tiles / w.pairs);
+    w.rest = (int)(tiles % w.pairs);
+    w.halves = w.rest > 0 && 2 * w.rest <= w.pairs;
+    return w;
+}
+
 // How many CTAs of a cluster share the sum over k of a tile, when single CTAs take tiles of 128 x (n per tile): as many as leave each
 // an SM of its own and four steps.
 inline int k_splits(int64_t tiles, int64_t steps, int sms) {
