@@ -336,7 +336,9 @@ struct PairArgs {
     int64_t m, n;
     uint32_t idesc;
     int64_t groups;
-    int m_tiles, n_tiles, tiles, ksteps, tma_out;
+    int m_tiles, n_tiles, ksteps, tma_out;
+    PairWork work;
+    uint32_t idesc_half;
     int ordered;              // the scale bytes have been put in order ahead
 };
 
@@ -372,7 +374,7 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
     uint8_t* smem = s_raw + ((1024 - (smem_u32(s_raw) & 1023)) & 1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
-    const int first = (int)(blockIdx.x >> 1), step = (int)(gridDim.x >> 1);
+    const int pair = (int)(blockIdx.x >> 1);
     if (warp == 8 && lane == 0) {
         for (int s = 0; s < S::kStages; ++s) { mbar_init(&full[s], (rank == 0 ? 2 : 1) + (a.ordered ? 0 : 8)); mbar_init(&empty[s], 1); }
         mbar_init(&acc_full, 1);
@@ -396,9 +398,11 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
     bool ok = true;   // a wait that ran out ends the role; what it would have computed is written as NaN
     if (warp == 8) {
         Slot<S::kStages> sl;
-        for (int t = first; t < a.tiles && ok; t += step) {
+        for (int i = 0, t, part; ok && a.work.piece(i, pair, t, part); ++i) {
             int tm, tn;
             tile_place(t, a.m_tiles, a.n_tiles, tm, tn);
+            // of a half tile each CTA brings 64 rows of B; the copy takes 64 more, which nobody reads
+            const int row_b = tn * 256 + (part < 0 ? rank * 128 : part * 128 + rank * 64), block_b = tn * 2 + (part > 0 ? 1 : 0);
             for (int j = 0; j < a.ksteps; ++j) {
                 ok = mbar_wait_warp(&empty[sl.s], sl.phase ^ 1);
                 if (!ok) break;
@@ -407,10 +411,10 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
                     uint64_t* bar = &full[sl.s];
                     mbar_expect_tx(bar, 2 * S::kTile + (a.ordered ? S::kSfP + S::kSfQ : 0));
                     tma_load_2d(st, &map_a, j * 128, tm * 256 + rank * 128, bar);
-                    tma_load_2d(st + S::kTile, &map_b, j * 128, tn * 256 + rank * 128, bar);
+                    tma_load_2d(st + S::kTile, &map_b, j * 128, row_b, bar);
                     if (a.ordered) {
                         tma_load_2d(st + S::kSfOff, &map_sa, j * (S::kBlk * 128), tm * 2 + rank, bar);
-                        tma_load_2d(st + S::kSfOff + S::kSfP, &map_sb, j * (S::kBlk * 128), tn * 2, bar);
+                        tma_load_2d(st + S::kSfOff + S::kSfP, &map_sb, j * (S::kBlk * 128), block_b, bar);
                     }
                 }
                 __syncwarp();
@@ -423,7 +427,7 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
         Slot<S::kStages> sl;
         if (rank == 1) {
             const uint32_t full0 = map_to_rank(smem_u32(&full[0]), 0);
-            const int64_t total = first < a.tiles ? (int64_t)((a.tiles - 1 - first) / step + 1) * a.ksteps : 0;
+            const int64_t total = (int64_t)a.work.pieces(pair) * a.ksteps;
             for (int64_t i = 0; i < total; ++i) {
                 if (!mbar_wait_warp(&full[sl.s], sl.phase)) break;
                 if (elect_one()) mbar_arrive_peer(full0 + 8 * sl.s);
@@ -432,8 +436,8 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
             }
         } else {
             const uint64_t d0 = umma_desc_kmajor(smem_u32(smem));
-            int it = 0;
-            for (int t = first; t < a.tiles && ok; t += step, ++it) {
+            for (int it = 0, t, part; ok && a.work.piece(it, pair, t, part); ++it) {
+                const uint32_t idesc = part < 0 ? a.idesc : a.idesc_half;
                 if (it > 0) ok = mbar_wait_warp(&acc_empty, (it - 1) & 1);
                 if (!ok) break;
                 for (int j = 0; j < a.ksteps; ++j) {
@@ -447,13 +451,13 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
                         for (int b = 0; b < S::kBlk; ++b) {   // a block is four groups of K: four columns for A's 128 rows, eight for B's 256
                             tc_copy_scales<2>(tp + 4 * b, sf + 512 * b);
                             tc_copy_scales<2>(tq + 8 * b, sf + S::kSfP + 512 * b);
-                            tc_copy_scales<2>(tq + 8 * b + 4, sf + 2 * S::kSfP + 512 * b);
+                            if (part < 0) tc_copy_scales<2>(tq + 8 * b + 4, sf + 2 * S::kSfP + 512 * b);
                         }
                         const uint64_t da = d0 + sl.s * (S::kStage / 16), db = da + S::kTile / 16;
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {   // 32 bytes of K each
                             const uint32_t blk = FP4 ? k >> 1 : 0, id = FP4 ? (k & 1) * 2 : k;
-                            tc_mma_scaled<2, FP4>(tmem, da + 2 * k, db + 2 * k, idesc_with_scale_id(a.idesc, id), tp + 4 * blk, tq + 8 * blk, (j | k) != 0);
+                            tc_mma_scaled<2, FP4>(tmem, da + 2 * k, db + 2 * k, idesc_with_scale_id(idesc, id), tp + 4 * blk, tq + 8 * blk, (j | k) != 0);
                         }
                         tc_commit_pair(&empty[sl.s]);
                         if (j == a.ksteps - 1) tc_commit_pair(&acc_full);
@@ -470,28 +474,29 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
         }
     } else {
         const int half = warp >> 2, t128 = threadIdx.x & 127;   // columns 128 half ..., accumulator row
-        const uint32_t acc = tmem + half * 128 + ((uint32_t)(warp & 3) << 21);
         const uint32_t empty0 = map_to_rank(smem_u32(&acc_empty), 0);
         uint8_t* os = smem + S::kOutOff + half * S::kOutBytes;
         if (!a.ordered) {   // the pair's only tile: these warps have nothing to write yet
-            int tm, tn;
-            tile_place(first, a.m_tiles, a.n_tiles, tm, tn);
+            int t, part, tm, tn;
+            a.work.piece(0, pair, t, part);
+            tile_place(t, a.m_tiles, a.n_tiles, tm, tn);
             constexpr int W = kBatch * S::kBlk;
-            const int64_t row_p = (int64_t)tm * 256 + rank * 128 + t128, row_q = (int64_t)tn * 256 + threadIdx.x;
+            const bool has_q = part < 0 || half == 0;
+            const int64_t row_p = (int64_t)tm * 256 + rank * 128 + t128, row_q = (int64_t)tn * 256 + (part > 0 ? 128 : 0) + threadIdx.x;
             const uint32_t sf = smem_u32(smem) + S::kSfOff + (t128 & 31) * 16 + (t128 >> 5) * 4, sfq = sf + S::kSfP * (1 + half);
             Slot<S::kStages> sl;
             ScaleWords<W> p, q, next_p, next_q;
             if (half == 0) p.load(a.sa, a.m, a.groups, row_p, 0);
-            q.load(a.sb, a.n, a.groups, row_q, 0);
+            if (has_q) q.load(a.sb, a.n, a.groups, row_q, 0);
             for (int i = 0; i < a.ksteps && ok; i += kBatch) {
                 if (i + kBatch < a.ksteps) {
                     const int64_t g = (int64_t)(i + kBatch) * (4 * S::kBlk);
                     if (half == 0) next_p.load(a.sa, a.m, a.groups, row_p, g);
-                    next_q.load(a.sb, a.n, a.groups, row_q, g);
+                    if (has_q) next_q.load(a.sb, a.n, a.groups, row_q, g);
                 }
                 uint32_t wp[W], wq[W];
                 if (half == 0) p.place(wp);
-                q.place(wq);
+                if (has_q) q.place(wq);
 #pragma unroll
                 for (int u = 0; u < kBatch; ++u) {
                     if (i + u >= a.ksteps) break;
@@ -500,7 +505,7 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
 #pragma unroll
                     for (int b = 0; b < S::kBlk; ++b) {
                         if (half == 0) store_word(sf + sl.s * S::kStage + 512 * b, wp[u * S::kBlk + b]);
-                        store_word(sfq + sl.s * S::kStage + 512 * b, wq[u * S::kBlk + b]);
+                        if (has_q) store_word(sfq + sl.s * S::kStage + 512 * b, wq[u * S::kBlk + b]);
                     }
                     fence_async_shared();
                     __syncwarp();
@@ -511,11 +516,12 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
                 q = next_q;
             }
         }
-        int it = 0;
-        for (int t = first; t < a.tiles; t += step, ++it) {
+        for (int it = 0, t, part; a.work.piece(it, pair, t, part); ++it) {
             int tm, tn;
             tile_place(t, a.m_tiles, a.n_tiles, tm, tn);
-            const int64_t m0 = (int64_t)tm * 256 + rank * 128, n0 = (int64_t)tn * 256 + half * 128;
+            const int columns = part < 0 ? 128 : 64;   // of these four warps
+            const uint32_t acc = tmem + half * columns + ((uint32_t)(warp & 3) << 21);
+            const int64_t m0 = (int64_t)tm * 256 + rank * 128, n0 = (int64_t)tn * 256 + (part > 0 ? 128 : 0) + half * columns;
             if (a.bias) {
                 named_barrier(1 + half, 128);   // the tile before is through with these
                 s_bias[half * 128 + t128] = n0 + t128 < a.n ? u2f((uint32_t)__ldg(a.bias + n0 + t128) << 16) : 0.0f;
@@ -526,6 +532,7 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
             uint32_t w[64];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
+                if (32 * c >= columns) break;
                 uint32_t r[32];
                 tmem_load32(acc + 32 * c, r);
                 tmem_wait_loads();
@@ -549,13 +556,14 @@ __global__ void __launch_bounds__(320, 1) mx_matmul_pair_kernel(const __grid_con
             bool at_once = false;   // after the last tile the operands' shared memory is free: both 64 columns go out at once
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
+                if (64 * c >= columns) break;
                 uint8_t* to = c == 1 && at_once ? smem + half * S::kOutBytes : os;
                 if (c == 0 || !at_once) {
                     if (t128 == 0) bulk_wait_reads();
                     named_barrier(1 + half, 128);
                 }
                 const bool late = s_late[half] != 0;
-                if (c == 0) at_once = !late && t + step >= a.tiles;
+                if (c == 0) at_once = !late && it + 1 == a.work.pieces(pair);
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     const uint32_t* v = w + 32 * c + 4 * q;
@@ -620,10 +628,11 @@ int go_pair(const MxMatmulArgs& x, cudaStream_t st) {
     a.m = x.m; a.n = x.n;
     a.m_tiles = (int)((x.m + 255) / 256); a.n_tiles = (int)((x.n + 255) / 256);
     if ((int64_t)a.m_tiles * a.n_tiles > (1 << 30)) return kErrTooLarge;
-    a.tiles = a.m_tiles * a.n_tiles;
+    a.work = pair_work((int64_t)a.m_tiles * a.n_tiles, sm_count());
     const int64_t row_bytes = FP4 ? x.k / 2 : x.k;
     a.ksteps = (int)((row_bytes + 127) / 128);
     a.idesc = idesc_scaled(256, 256, FP4 ? 1u : (uint32_t)x.a_fmt, FP4 ? 1u : (uint32_t)x.b_fmt);
+    a.idesc_half = idesc_scaled(256, 128, FP4 ? 1u : (uint32_t)x.a_fmt, FP4 ? 1u : (uint32_t)x.b_fmt);
     a.tma_out = x.n % 8 == 0 && (reinterpret_cast<uintptr_t>(x.out) & 15) == 0;
     CUtensorMap ma, mb, msa, msb, mo;
     if (!make_swizzled_map(&ma, x.a, x.m, row_bytes, row_bytes, 1, 128) || !make_swizzled_map(&mb, x.b, x.n, row_bytes, row_bytes, 1, 128)) return kErrLaunch;
@@ -635,7 +644,7 @@ int go_pair(const MxMatmulArgs& x, cudaStream_t st) {
     if (!a.ordered) msa = msb = ma;   // not used
     else if (!order_scales(x, S::kBlk, &msa, &msb, st)) return kErrLaunch;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(2 * std::min(a.tiles, sm_count() / 2)));
+    cfg.gridDim = dim3((unsigned)(2 * a.work.launched()));
     cfg.blockDim = dim3(320);
     cfg.dynamicSmemBytes = S::kSmem;
     cfg.stream = st;
