@@ -12,8 +12,8 @@
 // so every widened element meets 256 rows.
 //
 // A step of a pair is 0.287 us of the tensor core; widening 64 x 128 codes in the same time takes the integer pipe to 46 %
-// and the shared-memory pipe to 62 %.  8192 x 4096 x 4096 E4M3: 194 us in a short run (1.42 PFLOP/s, tensor pipe 73 %
-// active), 213 to 224 us in a long one (power limit).  One widening group of eight warps takes 27 % longer than two, three
+// and the shared-memory pipe to 62 %.  8192 x 4096 x 4096 E4M3: 190 us in a short run (1.45 PFLOP/s, tensor pipe 73 %
+// active), 213 to 221 us in a long one (power limit).  One widening group of eight warps takes 27 % longer than two, three
 // groups of four are best: what counts is that a group's waits hide behind the others' work.
 #include <algorithm>
 #include <type_traits>

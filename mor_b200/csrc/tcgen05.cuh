@@ -254,7 +254,8 @@ __device__ __forceinline__ void tile_place(int t, int m_tiles, int n_tiles, int&
 }
 
 // The work of the pairs of CTAs on 256 x 256 tiles: `rounds` whole tiles each, then the tiles that are left, as halves of 128
-// columns where there are pairs for them: a last round of few tiles then takes a little over half as long.
+// columns where there are pairs for them: 1024^3 E4M3 (16 tiles) 7.9 us in whole tiles, 6.7 in halves; gradient 512 x 4096 x
+// 4096 27.1 and 23.9; 2560 x 2560 x 8192 4-bit (100 tiles) 28.1 and 26.2.
 struct PairWork {
     int pairs, rounds, rest, halves;
     __host__ __device__ int launched() const { return rounds ? pairs : (halves ? 2 * rest : rest); }
@@ -290,13 +291,13 @@ inline int k_splits(int64_t tiles, int64_t steps, int sms) {
 }
 // Pairs of CTAs on 256 x 256 or single ones on 128 x 128?  A pair takes a step in about the time of a single CTA with four
 // times the result, so pairs win unless few tiles let single CTAs split the sum: each step saved is worth about 0.3 us,
-// meeting in the cluster costs about 3.  Measured on both sides, pairs and single, in us (steps saved): 128 x 4096 x 4096
-// E4M3 15.6 and 12.1 (24), 4-bit 11.6 and 11.0 (12); 256 x 4096 x 4096 E4M3 15.7 and 14.0 (16), 4-bit 11.7 and 12.0 (8);
-// 512 x 1024 x 8192 E4M3 25.5 and 14.9 (48); 1111 x 1003 x 2080 4-bit 11.7 and 12.6 (5); 1536 x 1536 x 4096 E4M3 16.1 and
-// 20.1 (0); gradients 128 x 4096 x 4096 27.2 and 17.0 (48), 1024^3 10.9 and 12.3 (8).
+// meeting in the cluster costs about 4.  Measured on both sides, pairs and single, in us (steps saved): 128 x 4096 x 4096
+// E4M3 14.2 and 12.0 (24), 4-bit 10.6 and 10.9 (12); 256 x 4096 x 4096 E4M3 14.2 and 13.8 (16), 4-bit 10.6 and 11.7 (8);
+// 512 x 1024 x 8192 E4M3 24.3 and 14.6 (48); 100 x 8192 x 8192 4-bit 17.7 and 15.2 (16); 1111 x 1003 x 2080 4-bit 10.3 and
+// 12.6 (5); 1536 x 1536 x 4096 E4M3 15.0 and 19.1 (0); gradients 128 x 4096 x 4096 23.0 and 16.9 (48), 1024^3 9.7 and 12.2 (8).
 inline bool takes_pairs(int64_t m, int64_t n, int64_t steps, int sms) {
     const int s = k_splits(((m + 127) / 128) * ((n + 127) / 128), steps, sms);
-    return steps - steps / s < 12;
+    return steps - steps / s < 14;
 }
 
 // row-major matrix of bytes (or bf16) with a row pitch, boxes of 128 bytes x box_rows under the 128-byte swizzle; what lies outside reads as zero
