@@ -202,6 +202,41 @@ def test_product_nan_scales_and_extremes(m, fmt):
     assert not bool(ops().mx_matmul(z.cuda(), torch.full_like(a[1], 127).cuda(), b[0][:100].cuda(), b[1][:100].cuda(), m, 100, k, fmt, fmt).any())
 
 
+def same_class(got, exact):
+    """NaN and infinities where the exact result has them, and nowhere else"""
+    got = got.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(exact))
+    assert torch.equal(torch.where(torch.isinf(got), got, 0.0), torch.where(torch.isinf(exact), exact, 0.0))
+
+
+@pytest.mark.parametrize("m", [6, 140, 4000])
+@pytest.mark.parametrize("fa,fb", [(E4M3, E4M3), (E5M2, E4M3), (E5M2, E5M2)])
+def test_product_codes_that_are_no_number(m, fa, fb):
+    n, k = 700, 256
+    a, b, _ = product_case(m, n, k, fa, fb, 5, False)
+    b[0][:] = torch.where((b[0] & 0x7F) == 0, torch.full_like(b[0], 0x30), b[0])     # no zero meets an infinity
+    a[0][1, 3], a[0][m - 1, 200] = 0x7F, 0xFF
+    b[0][n - 1, 17] = 0x7F
+    if fa == E5M2:
+        a[0][3, 100], a[0][4, 101] = 0x7C, 0xFC
+    bias = torch.zeros(n, dtype=torch.bfloat16)
+    bias[5], bias[6] = float("nan"), float("-inf")
+    got = ops().mx_matmul(*(t.cuda() for t in (*a, *b)), m, n, k, fa, fb, bias.cuda())
+    same_class(got, (R.decode(*a, fa) @ R.decode(*b, fb).t()) + bias.double())
+
+
+@pytest.mark.parametrize("across", [False, True])
+@pytest.mark.parametrize("m,n,k", [(40, 64, 100), (2400, 1312, 90)])
+def test_gradients_that_are_no_number(m, n, k, across):
+    """spoil their own rows of the result and nothing else, zeros behind the last k included"""
+    g = torch.randn(m, k, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    g[3, 7], g[m - 1, k - 1], g[5, 0], g[6, k - 1] = float("nan"), float("inf"), float("-inf"), float("inf")
+    w = R.random_codes(k, n, E4M3, 2)
+    w[0][:] = torch.where((w[0] & 0x7F) == 0, torch.full_like(w[0], 0x30), w[0])
+    got = ops().mx_matmul_grad((g.t().contiguous() if across else g).cuda(), w[0].cuda(), w[1].cuda(), m, n, k, E4M3, across)
+    same_class(got, g.double() @ R.decode(*w, E4M3))
+
+
 def test_product_empty():
     p, s = R.random_codes(4, 64, E4M3, 0)
     e = torch.empty(0, 64, dtype=torch.uint8), torch.empty(0, 2, dtype=torch.uint8)
