@@ -13,8 +13,8 @@
 //
 // A step of a pair is 0.287 us of the tensor core; widening 64 x 128 codes in the same time takes the integer pipe to 46 %
 // and the shared-memory pipe to 62 %.  8192 x 4096 x 4096 E4M3: 190 us in a short run (1.45 PFLOP/s, tensor pipe 73 %
-// active), 213 to 221 us in a long one (power limit).  One widening group of eight warps takes 27 % longer than two, three
-// groups of four are best: what counts is that a group's waits hide behind the others' work.
+// active), 213 to 221 us in a long one (power limit).  Two widening groups of four warps take 207 us, three
+// 193, four 193 (4096^3 4-bit: 139, 120, 116): what counts is that a group's waits hide behind the others' work.
 #include <algorithm>
 #include <type_traits>
 
@@ -35,7 +35,7 @@ struct GrArgs {
 
 constexpr int kTK = 64;                 // k a step: 128 bytes of bf16
 constexpr int kABytes = 128 * kTK * 2;  // a CTA's rows of the gradient
-constexpr int kConvWarps = 4, kConvGroups = 3;   // warps that widen a step together; the groups take the steps in turn
+constexpr int kConvWarps = 4, kConvGroups = 4;   // warps that widen a step together; the groups take the steps in turn
 constexpr int kFirstConv = 9;                    // warps 0-3 write, 4 gradient, 5 products, 6 codes, 7-8 scales
 constexpr int kThreads = 32 * (kFirstConv + kConvWarps * kConvGroups);
 
@@ -45,7 +45,7 @@ struct GrShape {
     static constexpr int kRowBytes = FMT == kE2M1 ? NB / 2 : NB;   // codes of one k
     static constexpr int kBBytes = NB * kTK * 2;
     static constexpr int kCodeBytes = kRowBytes * kTK, kCStage = kCodeBytes + kTK * 4;   // and their scale bytes
-    static constexpr int kSA = 4, kSB = 4, kSC = 5;                // depths of the rings
+    static constexpr int kSA = 4, kSB = 4, kSC = 6;                // depths of the rings
     static constexpr int kBOff = kSA * kABytes, kCOff = kBOff + kSB * kBBytes;
     static constexpr int kOutOff = kCOff + ((kSC * kCStage + 1023) & ~1023), kOutBytes = 128 * 128;   // two tiles of 128 x 64 on their way out
     static constexpr int kSmem = kOutOff + 2 * kOutBytes + 1024;
