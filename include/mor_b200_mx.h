@@ -65,6 +65,10 @@ MOR_B200_MX_API int mor_b200_mx_matmul(const void* a, const void* a_scales, cons
 MOR_B200_MX_API int mor_b200_mx_matmul_grad(const void* g, int64_t g_pitch, const void* payload, const void* scales, int64_t m,
                                             int64_t n, int64_t k, int format, int transpose_g, void* out, void* stream);
 
+/* out[c] = sum_r g[r, c]: the gradient of a bias.  g: bf16 [rows, cols], `pitch` elements from row to row (16-byte aligned,
+ * pitch a multiple of 8); out: bf16 [cols].  Sums in binary32 in a fixed order, rounded once; no rows give zeros. */
+MOR_B200_MX_API int mor_b200_mx_column_sums(const void* g, int64_t pitch, int64_t rows, int64_t cols, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

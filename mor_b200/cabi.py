@@ -66,6 +66,7 @@ MX_SIGNATURES = {
     "mor_b200_mx_dequantize": (_i, [_vp, _vp, _vp, _i, _i64, _i64, _i, _i, _vp]),
     "mor_b200_mx_matmul_workspace_bytes": (_sz, [_i64, _i64, _i64, _i]),
     "mor_b200_mx_matmul": (_i, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i, _i, _vp, _vp, _vp, _sz, _vp]),
+    "mor_b200_mx_column_sums": (_i, [_vp, _i64, _i64, _i64, _vp, _vp]),
     "mor_b200_mx_matmul_grad": (_i, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i, _i, _vp, _vp]),
 }
 

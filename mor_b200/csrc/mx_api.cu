@@ -85,4 +85,13 @@ int mor_b200_mx_matmul_grad(const void* g, int64_t g_pitch, const void* payload,
     return launch_mx_grad(x, static_cast<cudaStream_t>(stream));
 }
 
+int mor_b200_mx_column_sums(const void* g, int64_t pitch, int64_t rows, int64_t cols, void* out, void* stream) {
+    if (rows < 0 || cols < 0 || pitch < cols) return kErrInvalidArgument;
+    if (cols == 0) return kOk;
+    if (!out || (rows > 0 && !g)) return kErrInvalidArgument;
+    if (too_large(rows) || too_large(cols) || too_large(pitch)) return kErrTooLarge;
+    if ((rows > 1 && pitch % 8) || !aligned(g, 16) || !aligned(out, 2)) return kErrUnsupportedShape;
+    return launch_column_sums(g, pitch, rows, cols, out, static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

@@ -11,6 +11,8 @@ enum : int { kE2M1 = 4 };   // beside Fmt: two codes to a byte
 // mx_quant.cu
 int launch_quantize_fp4(const void* in, int is_fp32, int64_t rows, int64_t cols, int64_t pitch, void* payload, uint8_t* scales, cudaStream_t st);
 int launch_dequantize(const void* payload, const uint8_t* scales, void* out, int out_fp32, int64_t rows, int64_t cols, int bcols, int fmt, cudaStream_t st);
+// out[c] = sum_r g[r, c], bf16, rows `pitch` elements apart
+int launch_column_sums(const void* g, int64_t pitch, int64_t rows, int64_t cols, void* out, cudaStream_t st);
 
 // mx_matmul.cu: out[m, n] = sum_k a[m, k] b[n, k] + bias[n]
 struct MxMatmulArgs {

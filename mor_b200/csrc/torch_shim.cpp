@@ -366,6 +366,19 @@ at::Tensor mx_rows(const at::Tensor& t, int64_t& pitch) {
     return p;
 }
 
+at::Tensor column_sums(const at::Tensor& input, int64_t rows, int64_t cols) {
+    TORCH_CHECK(input.is_cuda(), "mor::column_sums: input must be a CUDA tensor");
+    const c10::cuda::CUDAGuard guard(input.device());
+    TORCH_CHECK(input.dim() == 2 && input.size(0) == rows && input.size(1) == cols, "mor::column_sums: input must be [dim_x, dim_y] = [",
+                rows, ", ", cols, "]");
+    TORCH_CHECK(input.scalar_type() == at::kBFloat16, "mor::column_sums: input must be bfloat16");
+    at::Tensor out = mx_empty({cols}, at::kBFloat16, input);
+    int64_t pitch = 0;
+    at::Tensor in = mx_rows(input, pitch);
+    check_status(mor_b200_mx_column_sums(in.data_ptr(), pitch, rows, cols, out.data_ptr(), cur_stream()), "column_sums");
+    return out;
+}
+
 // returns [payload uint8 [dim_x, dim_y / 2], scales uint8 [dim_x, dim_y / 32]]
 std::vector<at::Tensor> quantize_mx_fp4(const at::Tensor& input, int64_t rows, int64_t cols, int64_t bc) {
     TORCH_CHECK(input.is_cuda(), "mor::quantize_mx_fp4: input must be a CUDA tensor");
@@ -495,6 +508,8 @@ struct MxLinear : public torch::autograd::Function<MxLinear> {
         const int64_t k = sizes.back();
         at::Tensor g = grads[0].dim() == 2 ? grads[0] : grads[0].reshape({-1, n});
         const int64_t m = g.size(0);
+        int64_t pitch = 0;
+        g = mx_rows(g, pitch).narrow(1, 0, n);   // packed once where its rows do not fit, for all that read it
         auto typed = [](at::Tensor t, int64_t type) { return t.scalar_type() == (at::ScalarType)type ? t : t.to((at::ScalarType)type); };
         at::Tensor gx, gw, gb;
         if (kept[0].defined()) {
@@ -502,7 +517,7 @@ struct MxLinear : public torch::autograd::Function<MxLinear> {
             if (sizes.size() != 2) gx = gx.reshape(sizes);
         }
         if (kept[2].defined()) gw = typed(mx_matmul_grad(g, kept[2], kept[3], n, k, m, format, true), types[1]);
-        if (types[2] && ctx->needs_input_grad(2)) gb = typed(g.sum(0), types[2]);
+        if (types[2] && ctx->needs_input_grad(2)) gb = typed(column_sums(g, m, n), types[2]);
         return {gx, gw, gb, at::Tensor()};
     }
 };
@@ -566,6 +581,7 @@ TORCH_LIBRARY(mor, m) {
   m.def("dequantize_mx(Tensor payload, Tensor scales, int dim_x, int dim_y, int block_y, int elem_format, ScalarType out_dtype) -> Tensor");
   m.def("mx_matmul(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, int dim_m, int dim_n, int dim_k, int a_format, int b_format, Tensor? bias) -> Tensor");
   m.def("mx_matmul_grad(Tensor g, Tensor payload, Tensor scales, int dim_m, int dim_n, int dim_k, int elem_format, bool transpose_g) -> Tensor");
+  m.def("column_sums(Tensor input, int dim_x, int dim_y) -> Tensor");
   m.def("mx_linear(Tensor x, Tensor weight, Tensor? bias, int elem_format) -> Tensor", &mx_linear);   // composed of the above, with its gradient
   m.def("mx_linear_packed(Tensor x, Tensor payload, Tensor scales, Tensor? bias, int elem_format) -> Tensor", &mx_linear_packed);
 }
@@ -592,6 +608,7 @@ TORCH_LIBRARY_IMPL(mor, CUDA, m) {
   m.impl("fake_quantize_block_scaling_delayed", &fake_quantize_block_scaling_delayed);
   m.impl("fake_quantize_block_scaling_delayed_t", &fake_quantize_block_scaling_delayed_t);
   m.impl("quantize_mx_fp4", &quantize_mx_fp4);
+  m.impl("column_sums", &column_sums);
   m.impl("dequantize_mx", &dequantize_mx);
   m.impl("mx_matmul", &mx_matmul);
   m.impl("mx_matmul_grad", &mx_matmul_grad);

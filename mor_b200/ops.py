@@ -29,7 +29,7 @@ __all__ = [
     "quantize_scaled",
     "fake_quantize_block_scaling_delayed",
     "fake_quantize_block_scaling_delayed_t",
-    "quantize_mx_fp4", "dequantize_mx", "mx_matmul", "mx_matmul_grad",
+    "quantize_mx_fp4", "dequantize_mx", "mx_matmul", "mx_matmul_grad", "column_sums",
 ]
 
 
@@ -208,6 +208,12 @@ def mx_matmul_grad(g: Tensor, payload: Tensor, scales: Tensor, dim_m: int, dim_n
     matrix W ``[dim_k, dim_n]`` with groups of 32 columns, format 0, 1, 3 or 4: the input gradient of a linear layer from
     its quantised weights, and its weight gradient from the quantised input that the forward pass kept."""
     return _ops.mx_matmul_grad.default(g, payload, scales, dim_m, dim_n, dim_k, elem_format, transpose_g)
+
+
+def column_sums(a: Tensor, dim_x: int, dim_y: int) -> Tensor:
+    """Sums over the rows of a bfloat16 tensor, as bfloat16 ``[dim_y]``: the gradient of a linear layer's bias.  Sums in
+    binary32 in a fixed order, one rounding.  No gradient."""
+    return _ops.column_sums.default(a, dim_x, dim_y)
 
 
 # --------------------------------------------------------------------------- straight-through backward

@@ -404,6 +404,34 @@ def test_gradient_rows_beyond_the_result_are_left_alone():
         assert torch.equal(out[:m * n].view(m, n), ops().mx_matmul_grad(g[:, :k], c, s, m, n, k, 0, False))
 
 
+# ------------------------------------------------------------------------------------------------ column sums
+@pytest.mark.parametrize("rows,cols", [(0, 40), (1, 1), (1, 64), (3, 8), (31, 65), (33, 7), (127, 72), (128, 64), (141, 232), (513, 1003), (5003, 64),
+                                       (4096, 4096), (300, 8192), (70000, 24)])
+def test_column_sums(rows, cols):
+    g = torch.randn(rows, cols, generator=torch.Generator().manual_seed(rows)).to(torch.bfloat16)
+    got = ops().column_sums(g.cuda(), rows, cols)
+    assert got.shape == (cols,) and got.dtype == torch.bfloat16
+    exact, size = g.double().sum(0), g.double().abs().sum(0)
+    # one rounding of the result, and half a step of binary32 of what has been added up for each addition
+    assert bool(((got.double().cpu() - exact).abs() <= 2.0 ** -8 * exact.abs() + rows * 2.0 ** -24 * size + 2.0 ** -133).all())
+    assert torch.equal(got, ops().column_sums(g.cuda(), rows, cols))
+
+
+def test_column_sums_strides_and_refusals():
+    o = ops()
+    wide = torch.randn(200, 96, device="cuda").to(torch.bfloat16)
+    for v in (wide[:, 8:72], wide[:, 1:64], wide.t(), wide[::2, :40], wide[:1].expand(50, 96), wide[3:4]):
+        exact = v.double().sum(0)
+        assert bool(((o.column_sums(v, *v.shape).double() - exact).abs() <= 2.0 ** -8 * exact.abs() + 200 * 2.0 ** -24 * v.double().abs().sum(0)).all())
+    x = wide.clone()
+    x[5, 3], x[6, 4] = float("nan"), float("inf")
+    s = o.column_sums(x, 200, 96)
+    assert bool(torch.isnan(s[3])) and bool(torch.isinf(s[4])) and bool(torch.isfinite(s[5:]).all())
+    for bad in (lambda: o.column_sums(wide.float(), 200, 96), lambda: o.column_sums(wide, 100, 96), lambda: o.column_sums(wide[0], 1, 96)):
+        with pytest.raises(RuntimeError):
+            bad()
+
+
 # ------------------------------------------------------------------------------------------------ more than 2^31 elements
 def test_quantisation_past_32_bits():
     r, c = 70000, 32768

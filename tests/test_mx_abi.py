@@ -19,7 +19,7 @@ def declared():
 
 
 def test_header_library_and_binding_agree():
-    assert len(declared()) == 5
+    assert len(declared()) == 6
     out = subprocess.run(["nm", "-D", "--defined-only", cabi.MX_LIB_PATH], capture_output=True, text=True).stdout
     assert sorted(l.split()[-1] for l in out.splitlines() if " T " in l) == declared()
     assert sorted(cabi.MX_SIGNATURES) == declared()
@@ -111,6 +111,11 @@ def test_argument_errors_come_back_as_status_codes():
     assert g(p, 64, p, p, 4, 64, 0, 0, 0, None, None) == -1   # no sum, and nowhere to write the zeros
     assert g(p, 1 << 40, p, p, 4, 64, 64, 0, 0, p, None) == -5
     assert g(None, 64, None, None, 0, 64, 64, 0, 0, None, None) == 0
+
+    c = L.mor_b200_mx_column_sums
+    assert c(None, 64, 4, 64, p, None) == -1 and c(p, 64, 4, 64, None, None) == -1 and c(p, 32, 4, 64, p, None) == -1
+    assert c(p, 68, 4, 64, p, None) == -2 and c(p + 2, 64, 4, 64, p, None) == -2 and c(p, 64, 4, 64, p + 1, None) == -2
+    assert c(p, 1 << 40, 4, 64, p, None) == -5 and c(None, 0, 4, 0, None, None) == 0
 
 
 def test_schemas_and_cpu_tensors():
