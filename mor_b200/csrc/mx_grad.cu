@@ -12,9 +12,9 @@
 // so every widened element meets 256 rows.
 //
 // A step of a pair is 0.287 us of the tensor core; widening 64 x 128 codes in the same time takes the integer pipe to 46 %
-// and the shared-memory pipe to 62 %.  8192 x 4096 x 4096 E4M3: 190 us in a short run (1.45 PFLOP/s, tensor pipe 73 %
+// and the shared-memory pipe to 62 %.  8192 x 4096 x 4096 E4M3: 188 us in a short run (1.46 PFLOP/s, tensor pipe 73 %
 // active), 213 to 221 us in a long one (power limit).  Two widening groups of four warps take 207 us, three
-// 193, four 193 (4096^3 4-bit: 139, 120, 116): what counts is that a group's waits hide behind the others' work.
+// 187, four 188 (4096^3 4-bit: 139, 121, 116): what counts is that a group's waits hide behind the others' work.
 #include <algorithm>
 #include <type_traits>
 
@@ -45,7 +45,7 @@ struct GrShape {
     static constexpr int kRowBytes = FMT == kE2M1 ? NB / 2 : NB;   // codes of one k
     static constexpr int kBBytes = NB * kTK * 2;
     static constexpr int kCodeBytes = kRowBytes * kTK, kCStage = kCodeBytes + kTK * 4;   // and their scale bytes
-    static constexpr int kSA = 4, kSB = 4, kSC = 6;                // depths of the rings
+    static constexpr int kSA = 4, kSB = 4, kSC = 4;                // depths of the rings
     static constexpr int kBOff = kSA * kABytes, kCOff = kBOff + kSB * kBBytes;
     static constexpr int kOutOff = kCOff + ((kSC * kCStage + 1023) & ~1023), kOutBytes = 128 * 128;   // two tiles of 128 x 64 on their way out
     static constexpr int kSmem = kOutOff + 2 * kOutBytes + 1024;
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
                     }
                     asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst), "r"(w) : "memory");
                 }
-                cp_async_arrive(&full_c[sc.s]);
+                if (a.fast_scales) cp_async_arrive(&full_c[sc.s]); else mbar_arrive(&full_c[sc.s]);
                 sc.advance();
                 src += stride;
                 left -= kTK;
@@ -347,7 +347,11 @@ __global__ void __launch_bounds__(kThreads, 1) mx_grad_kernel(const __grid_const
             sb.advance(kConvGroups);
             sc.advance(kConvGroups);
         }
-        static_assert(kRowsPerPass % 8 == 0 && kConvGroups <= S::kSA && kConvGroups <= S::kSB && kConvGroups <= S::kSC, "swizzle, first slots");
+        // A wait by parity passes when the barrier is a whole round behind.  A slot of codes belongs to one group, which has
+        // seen its round before; the other two rings are safe because a group that found its widened tile's slot free
+        // knows that the products of kSB steps ago, and all before them, are done.
+        static_assert(S::kSC % kConvGroups == 0 && S::kSA <= S::kSB && kConvGroups <= S::kSA, "parities");
+        static_assert(kRowsPerPass % 8 == 0, "swizzle");
     } else {
         const uint32_t sums_to = sums.place(threadIdx.x);
         const uint32_t empty0 = CG == 2 ? map_to_rank(smem_u32(&acc_empty[0]), 0) : smem_u32(&acc_empty[0]);

@@ -404,6 +404,43 @@ def test_gradient_rows_beyond_the_result_are_left_alone():
         assert torch.equal(out[:m * n].view(m, n), ops().mx_matmul_grad(g[:, :k], c, s, m, n, k, 0, False))
 
 
+@pytest.mark.parametrize("fmt", [E4M3, E5M2, E2M1])
+@pytest.mark.parametrize("m,n,k,across", [(2, 3200, 5488, True), (2, 3200, 5486, True), (2, 3200, 5488, False), (1, 128, 8192, True),
+                                          (2304, 1312, 2000, True), (1304, 1408, 4000, False)])
+def test_grad_repeats_beside_others(m, n, k, across, fmt):
+    """on three streams at once, where the loads of one call are late in any order: a step's codes may land before an
+    earlier step's, and a gradient of two rows, nearly all of whose tile lies outside, before either"""
+    g = torch.randn((k, m) if across else (m, k), generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    c, s = (t.cuda() for t in R.random_codes(k, n, fmt, 2))
+    want = check_grad(m, n, k, fmt, across, seed=2, g=g, w=(c.cpu(), s.cpu()))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(30):
+        outs = []
+        for st in streams:
+            with torch.cuda.stream(st):
+                outs.append(ops().mx_matmul_grad(g, c, s, m, n, k, fmt, across))
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("fmt", [E4M3, E2M1])
+@pytest.mark.parametrize("m,n,k", [(1, 3200, 5504), (40, 1000, 4128), (100, 2048, 8192), (1300, 1400, 2080), (2400, 2300, 1024)])
+def test_product_repeats_beside_others(m, n, k, fmt):
+    a, b, _ = product_case(m, n, k, fmt, fmt, 8, False)
+    args = [t.cuda() for t in (*a, *b)]
+    want = check_product(m, n, k, fmt, fmt, a=a, b=b)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(30):
+        outs = []
+        for st in streams:
+            with torch.cuda.stream(st):
+                outs.append(ops().mx_matmul(*args, m, n, k, fmt, fmt))
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+
+
 # ------------------------------------------------------------------------------------------------ column sums
 @pytest.mark.parametrize("rows,cols", [(0, 40), (1, 1), (1, 64), (3, 8), (31, 65), (33, 7), (127, 72), (128, 64), (141, 232), (513, 1003), (5003, 64),
                                        (4096, 4096), (300, 8192), (70000, 24)])
