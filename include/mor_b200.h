@@ -189,7 +189,12 @@ MOR_B200_API int mor_b200_block_scaling_delayed_t(const void* input, void* outpu
  * element = decode(code) * 2^(scale - 127); an all-zero group gets 127.  block_cols a power of
  * two from 8 to 256.  decode * scale equals the fake-quantized
  * output bit for bit, except where the code is zero under a scale below one (fake quantization
- * returns 2^(-e8-127) there, an artefact of its exponent-field arithmetic, :296-305). */
+ * returns 2^(-e8-127) there, an artefact of its exponent-field arithmetic, :296-305).  Like fake
+ * quantization it is for finite values: codes and scale of a group that holds an infinity or a NaN are
+ * finite numbers of no meaning.
+ * With MOR_B200_MX_OPERAND added to the format the result is for a product (mor_b200_mx.h): a group that
+ * holds an infinity or a NaN gets byte 255 (NaN) and codes of zero. */
+#define MOR_B200_MX_OPERAND 16
 MOR_B200_API int mor_b200_quantize_mx(const void* input, void* payload, void* scales, int64_t rows, int64_t cols,
                          int block_cols, int format, void* stream);
 

@@ -3,7 +3,7 @@
  * The operators of mor_b200.h quantise; these take the real quantised form further.  None has a counterpart in
  * boryiings/mor, whose operators only fake-quantize.  An MX matrix [rows, cols] is
  *   payload: one code per element -- a byte for E4M3 (format 0), E5M2 (1) and E2M3 (3; the code in the low six bits), as
- *            mor_b200_quantize_mx writes them, or half a byte for E2M1 (4): column 2j in bits 0-3, 2j + 1 in bits 4-7;
+ *            mor_b200_quantize_mx writes them (with MOR_B200_MX_OPERAND added to its format, for products), or half a byte for E2M1 (4): column 2j in bits 0-3, 2j + 1 in bits 4-7;
  *   scales:  one E8M0 byte for every `block_cols` consecutive columns of a row, row-major;
  *   element = decode(code) * 2^(scale - 127), NaN where the scale byte is 255.
  * All pointers are device pointers of the current device; tensors are row-major and, unless said otherwise, contiguous.

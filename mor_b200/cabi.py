@@ -18,6 +18,7 @@ MX_LIB_PATH = os.path.join(_HERE, "libmor_b200_mx.so")
 BF16, FP32 = 0, 1
 E4M3, E5M2, E3M2, E2M3 = 0, 1, 2, 3
 E2M1 = 4
+MX_OPERAND = 16   # added to the format of mor_b200_quantize_mx
 SF_FP32, SF_E8 = 1, 2
 OP_BLOCK_SCALING, OP_CHANNEL_SCALING, OP_E8MX, OP_AMAX_NNZ = 1, 2, 3, 4
 

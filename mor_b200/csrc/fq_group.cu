@@ -302,6 +302,19 @@ __device__ __forceinline__ uint2 mx_codes_one(const uint4& v, uint32_t& scale_by
     return make_uint2(codes_fix_zero_sign<FMT>(c[0] | (c[1] << 16)), codes_fix_zero_sign<FMT>(c[2] | (c[3] << 16)));
 }
 
+// The same for the operand of a product, which has to show what is no number: a group that holds an infinity or a NaN
+// gets byte 255, MX's NaN, and codes of zero.
+template <int FMT, int GS>
+__device__ __forceinline__ uint2 mx_operand_codes_one(const uint4& v, uint32_t& scale_byte) {
+    uint32_t p = vec_amax_pattern(v);
+#pragma unroll
+    for (int o = (1 << GS) >> 1; o > 0; o >>= 1) p = max(p, __shfl_xor_sync(0xFFFFFFFFu, p, o));
+    const uint2 c = mx_codes_one<FMT, GS>(v, scale_byte);
+    if (p < 0x7F80u) return c;
+    scale_byte = 255u;
+    return make_uint2(0u, 0u);
+}
+
 // eight codes of a vector: one byte each, or (PACK6) six bits each in 6 bytes, code i in bits
 // [6 i, 6 i + 6) of the little-endian 48-bit group
 template <bool PACK6>
@@ -318,7 +331,7 @@ __device__ __forceinline__ void store_codes(uint2* __restrict__ payload, int64_t
     }
 }
 
-template <int FMT, int GS, bool PACK6 = false>
+template <int FMT, int GS, bool PACK6 = false, bool OPERAND = false>
 __global__ void __launch_bounds__(32 * kMxWarps, 5)
 mx_quantize_kernel(const uint4* __restrict__ in, uint2* __restrict__ payload, uint8_t* __restrict__ scales, int64_t nvec) {
     extern __shared__ __align__(128) uint8_t s_ring[];  // [warp][stage][2 KiB]
@@ -329,6 +342,10 @@ mx_quantize_kernel(const uint4* __restrict__ in, uint2* __restrict__ payload, ui
     ws.start(s_ring + wid * (kMxStages * kMxChunkVec * 16), s_bar[wid], in, nvec * 16, gw, n_warps);
     const int64_t n_chunks = (nvec + kMxChunkVec - 1) / kMxChunkVec;
     const bool scale_lane = (lane & ((1 << GS) - 1)) == 0;
+    auto codes_of = [](const uint4& v, uint32_t& sb) {
+        if constexpr (OPERAND) return mx_operand_codes_one<FMT, GS>(v, sb);
+        else return mx_codes_one<FMT, GS>(v, sb);
+    };
     int st = 0;
     for (int64_t c = gw; c < n_chunks; c += n_warps) {
         const int64_t v0 = c * kMxChunkVec;
@@ -341,7 +358,7 @@ mx_quantize_kernel(const uint4* __restrict__ in, uint2* __restrict__ payload, ui
 #pragma unroll
             for (int r = 0; r < kMxChunkVec / 32; ++r) {
                 uint32_t sb;
-                const uint2 codes = mx_codes_one<FMT, GS>(chunk[r * 32], sb);
+                const uint2 codes = codes_of(chunk[r * 32], sb);
                 store_codes<PACK6>(payload, o + r * 32, codes);
                 if (scale_lane) sc[r * (32 >> GS)] = (uint8_t)sb;
             }
@@ -349,7 +366,7 @@ mx_quantize_kernel(const uint4* __restrict__ in, uint2* __restrict__ payload, ui
             for (int r = 0; r * 32 < nv; ++r) {
                 const bool inside = r * 32 + lane < nv;   // whole groups: a row is a multiple of them
                 uint32_t sb;
-                const uint2 codes = mx_codes_one<FMT, GS>(inside ? ld_stream(in + v0 + r * 32 + lane) : make_uint4(0u, 0u, 0u, 0u), sb);
+                const uint2 codes = codes_of(inside ? ld_stream(in + v0 + r * 32 + lane) : make_uint4(0u, 0u, 0u, 0u), sb);
                 if (inside) {
                     store_codes<PACK6>(payload, o + r * 32, codes);
                     if (scale_lane) sc[r * (32 >> GS)] = (uint8_t)sb;
@@ -536,8 +553,8 @@ int launch_fmt(const void* in, void* out, float* scales, int32_t* meta, int32_t 
 }  // namespace
 
 int launch_quantize_mx(const void* in, void* payload, uint8_t* scales, int64_t rows, int64_t cols, int bcols, int fmt,
-                       int pack6, cudaStream_t st) {
-    if (pack6 && fmt != kE2M3) return kErrInvalidArgument;
+                       int pack6, int operand, cudaStream_t st) {
+    if (pack6 && (fmt != kE2M3 || operand)) return kErrInvalidArgument;
     if (bcols % 8 || cols % bcols) return kErrUnsupportedShape;
     const int gvec = bcols / 8;
     const int64_t nvec = rows * cols / 8;
@@ -552,11 +569,15 @@ int launch_quantize_mx(const void* in, void* payload, uint8_t* scales, int64_t r
     if (grid < 1) grid = 1;
     auto* i4 = static_cast<const uint4*>(in);
     auto* p2 = static_cast<uint2*>(payload);
-#define MORB_Q(F, GS)                                                                                                \
+#define MORB_QM(F, GS, OPERAND)                                                                                      \
     do {                                                                                                             \
         static SmemOptIn opt;                                                                                        \
-        if (!opt(mx_quantize_kernel<F, GS>, kRing)) return kErrLaunch;                                               \
-        mx_quantize_kernel<F, GS><<<(unsigned)grid, 32 * kMxWarps, kRing, st>>>(i4, p2, scales, nvec);               \
+        if (!opt(mx_quantize_kernel<F, GS, false, OPERAND>, kRing)) return kErrLaunch;                               \
+        mx_quantize_kernel<F, GS, false, OPERAND><<<(unsigned)grid, 32 * kMxWarps, kRing, st>>>(i4, p2, scales, nvec); \
+    } while (0)
+#define MORB_Q(F, GS)                                                                                                \
+    do {                                                                                                             \
+        if (operand) MORB_QM(F, GS, true); else MORB_QM(F, GS, false);                                               \
     } while (0)
 #define MORB_QS(F)                                                                                                   \
     do {                                                                                                             \
@@ -591,6 +612,7 @@ int launch_quantize_mx(const void* in, void* payload, uint8_t* scales, int64_t r
 #undef MORB_Q6
 #undef MORB_QS
 #undef MORB_Q
+#undef MORB_QM
     return check_launch();
 }
 

@@ -285,7 +285,7 @@ std::vector<at::Tensor> fake_quantize_block_scaling_delayed_t(const at::Tensor& 
 
 // ---- extension: real quantized output (codes + E8M0 scale bytes) -----------------------
 // returns [payload uint8 [dim_x, dim_y], scales uint8 [dim_x, dim_y / block_y]]
-std::vector<at::Tensor> quantize_mx(const at::Tensor& input, int64_t rows, int64_t cols, int64_t bc, int64_t elem_format) {
+std::vector<at::Tensor> quantize_mx(const at::Tensor& input, int64_t rows, int64_t cols, int64_t bc, int64_t elem_format, bool operand) {
     const c10::cuda::CUDAGuard guard(input.device());
     at::Tensor in = checked_input(input, rows, cols, "quantize_mx");
     TORCH_CHECK(in.scalar_type() == at::kBFloat16, "mor::quantize_mx: bfloat16 input only");
@@ -295,7 +295,7 @@ std::vector<at::Tensor> quantize_mx(const at::Tensor& input, int64_t rows, int64
     at::Tensor payload = torch::empty({rows, cols}, in.options().dtype(torch::kUInt8));
     at::Tensor scales = torch::empty({rows, cols / bc}, in.options().dtype(torch::kUInt8));
     check_status(mor_b200_quantize_mx(in.data_ptr(), payload.data_ptr(), scales.data_ptr(), rows, cols, (int)bc,
-                                      (int)elem_format, cur_stream()),
+                                      (int)elem_format + (operand ? MOR_B200_MX_OPERAND : 0), cur_stream()),
                  "quantize_mx");
     return {payload, scales};
 }
@@ -472,7 +472,7 @@ std::vector<at::Tensor> mx_quantized(const at::Tensor& x, int64_t format) {
     if (r == 0) return {mx_empty({0, c}, at::kByte, x), mx_empty({0, c / 32}, at::kByte, x)};
     at::Tensor packed = x.contiguous();
     if (reinterpret_cast<uintptr_t>(packed.data_ptr()) % 16) packed = packed.clone();
-    return quantize_mx(packed, r, c, 32, format);
+    return quantize_mx(packed, r, c, 32, format, /*operand=*/true);
 }
 
 // Straight-through: the gradients are those of a linear layer fed the quantised values, computed from the codes, which are
@@ -571,7 +571,7 @@ TORCH_LIBRARY(mor, m) {
   m.def("fake_quantize_channel_scaling_inplace(Tensor input, int dim_x, int dim_y, int block_x, int block_y, float e4m3_threshold, int ss_mode) -> Tensor[]");
   // addition: one scale per 1 x block_y group (MX), E4M3 / E5M2 / E2M3 elements
   m.def("fake_quantize_mx(Tensor input, int dim_x, int dim_y, int block_y, int elem_format, int sf_type) -> Tensor[]");
-  m.def("quantize_mx(Tensor input, int dim_x, int dim_y, int block_y, int elem_format) -> Tensor[]");
+  m.def("quantize_mx(Tensor input, int dim_x, int dim_y, int block_y, int elem_format, bool operand=False) -> Tensor[]");
   m.def("quantize_mx_fp6(Tensor input, int dim_x, int dim_y, int block_y) -> Tensor[]");
   m.def("quantize_scaled(Tensor input, int dim_x, int dim_y, int block_x, int block_y, int ss_mode) -> Tensor[]");
   m.def("fake_quantize_block_scaling_delayed(Tensor input, int dim_x, int dim_y, int block_x, int block_y, float e4m3_threshold, int ss_mode, Tensor amax_in) -> Tensor[]");

@@ -192,13 +192,14 @@ MX_FORMATS = {"e4m3": 0, "e5m2": 1, "e2m1": 4}
 def _mx_quantize(x: Tensor, elem_format: int):
     """Codes and scale bytes of a ``[rows, cols]`` tensor in groups of 32 columns."""
     r, c = x.shape
-    return ops.quantize_mx_fp4(x, r, c, 32) if elem_format == 4 else ops.quantize_mx(x, r, c, 32, elem_format)
+    return ops.quantize_mx_fp4(x, r, c, 32) if elem_format == 4 else ops.quantize_mx(x, r, c, 32, elem_format, operand=True)
 
 
 def mx_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, elem_format: int = 0) -> Tensor:
     """``x @ weight.T + bias`` on microscaled operands: ``x`` ``[..., in]`` and ``weight`` ``[out, in]`` are quantised in
     groups of 32 along ``in`` (a multiple of 32) and multiplied as codes; the result is bfloat16.  ``elem_format``: 0 E4M3,
-    1 E5M2 (bfloat16 inputs), 4 E2M1 (bfloat16 or float32).  The gradients are straight-through: those of a linear layer
+    1 E5M2 (bfloat16 inputs), 4 E2M1 (bfloat16 or float32).  A group that holds an infinity or a NaN counts as NaN in whole,
+    in the product and in the gradients.  The gradients are straight-through: those of a linear layer
     fed the quantised values, computed from the codes, which are all that the forward pass keeps of ``x`` and ``weight``
     -- one byte (E2M1: half a byte) and a thirty-second per element in place of two; they have no gradient of their own.
     Each call quantises the weight it

@@ -153,12 +153,14 @@ def fake_quantize_block_scaling_delayed_t(a: Tensor, dim_x: int, dim_y: int, blo
     return _ops.fake_quantize_block_scaling_delayed_t.default(a, dim_x, dim_y, block_x, block_y, e4m3_threshold, ss_mode, amax_in)
 
 
-def quantize_mx(a: Tensor, dim_x: int, dim_y: int, block_y: int, elem_format: int) -> List[Tensor]:
+def quantize_mx(a: Tensor, dim_x: int, dim_y: int, block_y: int, elem_format: int, operand: bool = False) -> List[Tensor]:
     """The real quantized form of :func:`fake_quantize_mx` with a power-of-two scale: returns
     ``[payload, scales]``, both ``uint8``: one narrow-float code per element (fp8 byte for E4M3 / E5M2, the
     6-bit code in a byte for E2M3) and one E8M0 byte per 1 x ``block_y`` group;
-    ``element = decode(code) * 2 ** (scale - 127)``.  No gradient."""
-    return _ops.quantize_mx.default(a, dim_x, dim_y, block_y, elem_format)
+    ``element = decode(code) * 2 ** (scale - 127)``.  Like fake quantization it is for finite values; with
+    ``operand``, which is what :func:`mx_matmul` and :func:`mx_matmul_grad` should be given, a group that holds an infinity
+    or a NaN gets scale byte 255 (NaN), as :func:`quantize_mx_fp4` has it.  No gradient."""
+    return _ops.quantize_mx.default(a, dim_x, dim_y, block_y, elem_format, operand)
 
 
 def quantize_mx_fp6(a: Tensor, dim_x: int, dim_y: int, block_y: int) -> List[Tensor]:
