@@ -190,9 +190,12 @@ MOR_B200_API int mor_b200_block_scaling_delayed_t(const void* input, void* outpu
  * two from 8 to 256.  decode * scale equals the fake-quantized
  * output bit for bit, except where the code is zero under a scale below one (fake quantization
  * returns 2^(-e8-127) there, an artefact of its exponent-field arithmetic, :296-305).  Like fake
- * quantization it is for finite values: codes and scale of a group that holds an infinity or a NaN are
- * finite numbers of no meaning.
- * With MOR_B200_MX_OPERAND added to the format the result is for a product (mor_b200_mx.h): a group that
+ * quantization it is for finite values, codes and scale of a group that holds an infinity or a NaN are
+ * finite numbers of no meaning, and groups below about 2^-92 follow the field arithmetic: zeros among
+ * them may get the code of a small number, and the byte stops at 0 where the codes' scale does not.
+ * With MOR_B200_MX_OPERAND added to the format the result is for a product (mor_b200_mx.h): the byte is
+ * that of the largest power of two 2^(127 - byte) that keeps the group's largest magnitude within the
+ * format's, at least 0, and codes are the values under that scale rounded to nearest even; a group that
  * holds an infinity or a NaN gets byte 255 (NaN) and codes of zero. */
 #define MOR_B200_MX_OPERAND 16
 MOR_B200_API int mor_b200_quantize_mx(const void* input, void* payload, void* scales, int64_t rows, int64_t cols,

@@ -302,17 +302,29 @@ __device__ __forceinline__ uint2 mx_codes_one(const uint4& v, uint32_t& scale_by
     return make_uint2(codes_fix_zero_sign<FMT>(c[0] | (c[1] << 16)), codes_fix_zero_sign<FMT>(c[2] | (c[3] << 16)));
 }
 
-// The same for the operand of a product, which has to show what is no number: a group that holds an infinity or a NaN
-// gets byte 255, MX's NaN, and codes of zero.
+// The same for the operand of a product: what stands for a group is its values as nearly as the format has them, at every
+// magnitude.  The byte is limited to 0 first and the codes are made for the scale that it says, by a multiplication (exact
+// but for products below 2^-126, far below half the smallest code), so zeros stay zeros; a group that holds an infinity
+// or a NaN gets byte 255, MX's NaN, and codes of zero.  With amax = 1.m * 2^(ea - 127) the largest power of two that keeps
+// it at or below c * 2^k is 2^(127 - s), s = ea - k, one more where 1.m > c; amax is at most 2^128, so s <= 253 and no
+// factor is subnormal.  Groups that mx_codes_one takes on its short path get the same bytes from both.
+// Bound by memory: 16384 x 8192 E4M3 61.6 us = 6.6 TB/s (mx_codes_one 64.2), 4096 x 4096 9.4 (9.7), one row of 4096 2.1.
 template <int FMT, int GS>
 __device__ __forceinline__ uint2 mx_operand_codes_one(const uint4& v, uint32_t& scale_byte) {
+    constexpr int K = (FMT == kE4M3) ? 8 : (FMT == kE5M2 ? 15 : 2);
+    constexpr uint32_t CMAN7 = (FMT == kE2M3) ? 0x70u : 0x60u;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     uint32_t p = vec_amax_pattern(v);
 #pragma unroll
     for (int o = (1 << GS) >> 1; o > 0; o >>= 1) p = max(p, __shfl_xor_sync(0xFFFFFFFFu, p, o));
-    const uint2 c = mx_codes_one<FMT, GS>(v, scale_byte);
-    if (p < 0x7F80u) return c;
-    scale_byte = 255u;
-    return make_uint2(0u, 0u);
+    const int s = max((int)(p >> 7) - K + ((p & 0x7Fu) > CMAN7 ? 1 : 0), 0);
+    const float up = u2f((uint32_t)(254 - min(s, 253)) << 23);
+    uint32_t c[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) c[k] = cvt_codes<FMT>(__fmul_rn(bf16_hi(w[k]), up), __fmul_rn(bf16_lo(w[k]), up));
+    const bool number = p < 0x7F80u;
+    scale_byte = number ? (p == 0u ? 127u : (uint32_t)s) : 255u;
+    return number ? make_uint2(codes_fix_zero_sign<FMT>(c[0] | (c[1] << 16)), codes_fix_zero_sign<FMT>(c[2] | (c[3] << 16))) : make_uint2(0u, 0u);
 }
 
 // eight codes of a vector: one byte each, or (PACK6) six bits each in 6 bytes, code i in bits

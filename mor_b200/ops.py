@@ -157,9 +157,10 @@ def quantize_mx(a: Tensor, dim_x: int, dim_y: int, block_y: int, elem_format: in
     """The real quantized form of :func:`fake_quantize_mx` with a power-of-two scale: returns
     ``[payload, scales]``, both ``uint8``: one narrow-float code per element (fp8 byte for E4M3 / E5M2, the
     6-bit code in a byte for E2M3) and one E8M0 byte per 1 x ``block_y`` group;
-    ``element = decode(code) * 2 ** (scale - 127)``.  Like fake quantization it is for finite values; with
-    ``operand``, which is what :func:`mx_matmul` and :func:`mx_matmul_grad` should be given, a group that holds an infinity
-    or a NaN gets scale byte 255 (NaN), as :func:`quantize_mx_fp4` has it.  No gradient."""
+    ``element = decode(code) * 2 ** (scale - 127)``.  It keeps to fake quantization's
+    arithmetic, which is for finite values in groups above about ``2 ** -92``.  With ``operand``, which is what :func:`mx_matmul`
+    and :func:`mx_matmul_grad` should be given, codes are the nearest values at every magnitude, zeros stay zeros, and a group
+    that holds an infinity or a NaN gets scale byte 255 (NaN), as :func:`quantize_mx_fp4` has it.  No gradient."""
     return _ops.quantize_mx.default(a, dim_x, dim_y, block_y, elem_format, operand)
 
 

@@ -110,3 +110,60 @@ def test_operand_groups_that_hold_no_numbers(fmt, group):
     bad = (~torch.isfinite(spoiled)).reshape(37, -1, group).any(2)
     assert torch.equal(got[1].cpu(), torch.where(bad, 255, want[1].cpu()))
     assert torch.equal(got[0].cpu(), torch.where(bad.repeat_interleave(group, 1), 0, want[0].cpu()))
+
+
+# ------------------------------------------------------------------------------------------------ very small and large groups
+@pytest.mark.parametrize("name", FORMATS)
+@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("power", [-80, -100, -110, -114, -116, -120, -122, -126, -130])
+def test_small_groups(power, m, n, k, name):
+    """down to where the scale's byte is 0 and to subnormal inputs, zeros among them; the other operand large, so that the
+    products are ordinary numbers"""
+    x, w, b, g, gen = operands(m, n, k, m)
+    zeros = torch.rand(m, k, generator=gen) < 0.2
+    x[zeros] = 0.0
+    up, down = 2.0 ** 60, 2.0 ** power
+    check_step(x * down, w * up, b * down * up, g * up, name)
+    check_step(w * down, x * up, g[:, 0] * down * up, g.t() * up, name)
+
+
+@pytest.mark.parametrize("name", FORMATS)
+@pytest.mark.parametrize("kind,w_scale", [("tiny", 2.0 ** 60), ("huge", 2.0 ** -60), ("ties", 1.0), ("sparse", 1.0)])
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_values_of_every_size(m, n, k, kind, w_scale, name):
+    _, w, b, g, _ = operands(m, n, k, m)
+    check_step(values(kind, m, k, m, torch.float32), w * w_scale, b, g * w_scale, name)
+
+
+@pytest.mark.parametrize("fmt", [R.E4M3, R.E5M2, R.E2M3])
+@pytest.mark.parametrize("group", [8, 16, 32, 64, 128, 256])
+@pytest.mark.parametrize("kind", ["normal", "wide", "tiny", "huge", "ties", "sparse", "bad"])
+def test_operands_are_the_nearest_values(kind, group, fmt):
+    """scale bytes and values by the definition, bit for bit; the number of vectors is no multiple of a warp's"""
+    import mor
+    x = values(kind, 37, 768, 11, torch.bfloat16)
+    if kind == "tiny":
+        x[20:] *= 2.0 ** torch.linspace(0, 60, 17)[:, None]
+        x[:, ::5] = 0.0
+    codes, scales = mor.ops.quantize_mx(x.cuda(), 37, 768, group, fmt, operand=True)
+    want, bytes_ = quantised(x, fmt, group)
+    assert torch.equal(scales.cpu(), bytes_)
+    got = R.decode(codes, scales, fmt, group)
+    nan = torch.isnan(want)
+    assert torch.equal(torch.isnan(got), nan) and torch.equal(got[~nan], want[~nan])
+    assert not bool(codes.cpu()[nan].any())
+
+
+@pytest.mark.parametrize("fmt", [R.E4M3, R.E5M2, R.E2M3])
+def test_operands_of_ordinary_groups_keep_their_bytes(fmt):
+    """with and without the mode alike, at sizes of one group up to more than a round of blocks, and nothing behind them"""
+    import mor
+    from mor_b200 import cabi
+    for rows, cols in ((1, 32), (3, 32), (129, 96), (1000, 4128)):
+        x = (torch.randn(rows, cols, generator=torch.Generator().manual_seed(rows)) * 3).to(torch.bfloat16).cuda()
+        want = mor.ops.quantize_mx(x, rows, cols, 32, fmt)
+        got = [torch.full((t.numel() + 512,), 9, dtype=torch.uint8, device="cuda") for t in want]
+        cabi.call("mor_b200_quantize_mx", x.data_ptr(), got[0].data_ptr(), got[1].data_ptr(), rows, cols, 32, fmt + cabi.MX_OPERAND,
+                  torch.cuda.current_stream().cuda_stream)
+        for u, v in zip(got, want):
+            assert torch.equal(u[:v.numel()].view(v.shape), v) and bool((u[v.numel():] == 9).all())
