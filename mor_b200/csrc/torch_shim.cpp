@@ -512,11 +512,12 @@ struct MxLinear : public torch::autograd::Function<MxLinear> {
         g = mx_rows(g, pitch).narrow(1, 0, n);   // packed once where its rows do not fit, for all that read it
         auto typed = [](at::Tensor t, int64_t type) { return t.scalar_type() == (at::ScalarType)type ? t : t.to((at::ScalarType)type); };
         at::Tensor gx, gw, gb;
-        if (kept[0].defined()) {
+        // a gradient that this pass does not ask for costs a whole product
+        if (kept[0].defined() && ctx->needs_input_grad(0)) {
             gx = typed(mx_matmul_grad(g, kept[0], kept[1], m, k, n, format, false), types[0]);
             if (sizes.size() != 2) gx = gx.reshape(sizes);
         }
-        if (kept[2].defined()) gw = typed(mx_matmul_grad(g, kept[2], kept[3], n, k, m, format, true), types[1]);
+        if (kept[2].defined() && ctx->needs_input_grad(1)) gw = typed(mx_matmul_grad(g, kept[2], kept[3], n, k, m, format, true), types[1]);
         if (types[2] && ctx->needs_input_grad(2)) gb = typed(column_sums(g, m, n), types[2]);
         return {gx, gw, gb, at::Tensor()};
     }

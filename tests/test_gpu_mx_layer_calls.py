@@ -1,0 +1,29 @@
+"""Calls of the layer on microscaled operands as programs around it make them."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("name", ["e4m3", "e2m1"])
+def test_a_pass_computes_the_gradients_that_it_is_asked_for(name):
+    """the others are neither computed nor given memory; those asked for are the same bits as in a whole pass"""
+    from mor_b200.nn import MXLinear
+    torch.manual_seed(0)
+    layer = MXLinear(2048, 2048, device="cuda", elem_format=name)
+    x = torch.randn(2048, 2048, device="cuda").to(torch.bfloat16).requires_grad_()
+    leaves = {"x": x, "weight": layer.weight, "bias": layer.bias}
+    y = layer(x)
+    g = torch.randn_like(y)
+    whole = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), g, retain_graph=True)))
+    for asked in (("x",), ("weight",), ("bias",), ("x", "bias"), ("weight", "bias"), ("x", "weight")):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got = torch.autograd.grad(y, [leaves[a] for a in asked], g, retain_graph=True)
+        peak = torch.cuda.max_memory_allocated() - before
+        assert all(torch.equal(t, whole[a]) for t, a in zip(got, asked)), asked
+        assert peak < sum(whole[a].numel() * 2 for a in asked) + (1 << 20), (asked, peak)
+    layer.weight.grad = None
+    y.backward(g, inputs=[layer.weight])
+    assert torch.equal(layer.weight.grad, whole["weight"]) and x.grad is None and layer.bias.grad is None
