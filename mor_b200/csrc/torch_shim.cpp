@@ -475,6 +475,15 @@ std::vector<at::Tensor> mx_quantized(const at::Tensor& x, int64_t format) {
     return quantize_mx(packed, r, c, 32, format, /*operand=*/true);
 }
 
+// [tokens, n] in the shape of x but for its last dimension.  Not a view that autograd tracks: it is the only tensor on its memory, and
+// as a view made inside a custom function, or without gradients, it could not be written in place (relu_, y += ...).
+at::Tensor mx_shaped(const at::Tensor& y, at::IntArrayRef x_sizes) {
+    if (x_sizes.size() == 2) return y;
+    std::vector<int64_t> shape = x_sizes.vec();
+    shape.back() = y.size(1);
+    return at::_unsafe_view(y, shape);
+}
+
 // Straight-through: the gradients are those of a linear layer fed the quantised values, computed from the codes, which are
 // all that the forward pass keeps of the input and the weight.
 struct MxLinear : public torch::autograd::Function<MxLinear> {
@@ -495,10 +504,7 @@ struct MxLinear : public torch::autograd::Function<MxLinear> {
         ctx->saved_data["n"] = n;
         ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)x.scalar_type(), (int64_t)weight.scalar_type(),
                                                         b.has_value() ? (int64_t)bias->scalar_type() : 0};
-        if (x.dim() == 2) return y;
-        std::vector<int64_t> shape = x.sizes().vec();
-        shape.back() = n;
-        return y.reshape(shape);
+        return mx_shaped(y, x.sizes());
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "mor::mx_linear is differentiable once: its gradients have no gradient (create_graph)");
@@ -543,10 +549,7 @@ at::Tensor mx_linear_packed(const at::Tensor& x, const at::Tensor& payload, cons
     at::Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, k});
     const std::vector<at::Tensor> q = mx_quantized(x2, format);
     at::Tensor y = mx_matmul(q[0], q[1], payload, scales, x2.size(0), n, k, format, format, bias);
-    if (x.dim() == 2) return y;
-    std::vector<int64_t> shape = x.sizes().vec();
-    shape.back() = n;
-    return y.reshape(shape);
+    return mx_shaped(y, x.sizes());
 }
 
 }  // namespace

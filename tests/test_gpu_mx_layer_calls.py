@@ -27,3 +27,24 @@ def test_a_pass_computes_the_gradients_that_it_is_asked_for(name):
     layer.weight.grad = None
     y.backward(g, inputs=[layer.weight])
     assert torch.equal(layer.weight.grad, whole["weight"]) and x.grad is None and layer.bias.grad is None
+
+
+@pytest.mark.parametrize("name", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("shape", [(64,), (6, 64), (2, 3, 64), (2, 1, 3, 64), (0, 3, 64)])
+def test_results_can_be_written_in_place(shape, name):
+    """as those of torch's own layer can: an activation in place, a residual added"""
+    from mor_b200.nn import MXLinear
+    torch.manual_seed(0)
+    layer = MXLinear(64, 32, device="cuda", elem_format=name)
+    x = torch.randn(*shape, device="cuda").to(torch.bfloat16).requires_grad_()
+    r = torch.randn(*shape[:-1], 32, device="cuda").to(torch.bfloat16).requires_grad_()
+
+    def grads(f):
+        return torch.autograd.grad(f().float().sum(), (x, r, layer.weight, layer.bias), allow_unused=True)
+    for inside, beside in ((lambda: torch.relu_(layer(x)) + r, lambda: torch.relu(layer(x)) + r), (lambda: layer(x).add_(r), lambda: layer(x) + r)):
+        assert torch.equal(inside(), beside())
+        assert all(torch.equal(u, v) for u, v in zip(grads(inside), grads(beside)))
+    packed = layer.pack()
+    y = packed(x).add_(r)
+    assert y.shape == (*shape[:-1], 32) and torch.equal(y, packed(x) + r) and packed(x).is_contiguous()
+    assert torch.equal(torch.autograd.grad(y.float().sum(), r)[0], torch.ones_like(r))
