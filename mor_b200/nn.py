@@ -187,6 +187,7 @@ class MoRLinear(torch.nn.Linear):
 
 # --------------------------------------------------------------------------- linear layer on microscaled operands
 MX_FORMATS = {"e4m3": 0, "e5m2": 1, "e2m1": 4}
+MX_INPUT_TYPES = {"e4m3": (torch.bfloat16,), "e5m2": (torch.bfloat16,), "e2m1": (torch.bfloat16, torch.float32)}   # what is quantised to them
 
 
 def _mx_quantize(x: Tensor, elem_format: int):
@@ -212,7 +213,8 @@ def mx_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, elem_for
 
 
 class MXLinear(torch.nn.Linear):
-    """``torch.nn.Linear`` computed by :func:`mx_linear`; ``elem_format`` "e4m3", "e5m2" or "e2m1"."""
+    """``torch.nn.Linear`` computed by :func:`mx_linear`; ``elem_format`` "e4m3", "e5m2" (bfloat16) or "e2m1"
+    (bfloat16 or float32)."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=torch.bfloat16,
                  elem_format: str = "e4m3"):
@@ -220,6 +222,8 @@ class MXLinear(torch.nn.Linear):
             raise ValueError(f"elem_format must be one of {sorted(MX_FORMATS)}, got {elem_format!r}")
         if in_features % 32:
             raise ValueError(f"in_features must be a multiple of 32, got {in_features}")
+        if (dtype or torch.get_default_dtype()) not in MX_INPUT_TYPES[elem_format]:
+            raise ValueError(f"dtype for {elem_format} must be one of {MX_INPUT_TYPES[elem_format]}, got {dtype or torch.get_default_dtype()}")
         super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
         self.elem_format = elem_format
 
