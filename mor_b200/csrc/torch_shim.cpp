@@ -475,6 +475,12 @@ std::vector<at::Tensor> mx_quantized(const at::Tensor& x, int64_t format) {
     return quantize_mx(packed, r, c, 32, format, /*operand=*/true);
 }
 
+// A layer's bias as the product adds it: in binary32 before the result's rounding, from bf16, the result's own precision.
+std::optional<at::Tensor> mx_bias(const std::optional<at::Tensor>& bias) {
+    if (!bias.has_value() || !bias->defined() || bias->scalar_type() == at::kBFloat16) return bias;
+    return bias->to(at::kBFloat16);
+}
+
 // [tokens, n] in the shape of x but for its last dimension.  Not a view that autograd tracks: it is the only tensor on its memory, and
 // as a view made inside a custom function, or without gradients, it could not be written in place (relu_, y += ...).
 at::Tensor mx_shaped(const at::Tensor& y, at::IntArrayRef x_sizes) {
@@ -493,8 +499,7 @@ struct MxLinear : public torch::autograd::Function<MxLinear> {
         at::Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, k});
         const int64_t m = x2.size(0);
         const std::vector<at::Tensor> xq = mx_quantized(x2, format), wq = mx_quantized(weight, format);
-        std::optional<at::Tensor> b;
-        if (bias.has_value() && bias->defined()) b = bias->scalar_type() == at::kBFloat16 ? *bias : bias->to(at::kBFloat16);
+        const std::optional<at::Tensor> b = mx_bias(bias);
         at::Tensor y = mx_matmul(xq[0], xq[1], wq[0], wq[1], m, n, k, format, format, b);
         const bool need_x = x.requires_grad(), need_w = weight.requires_grad();
         ctx->save_for_backward({need_x ? wq[0] : at::Tensor(), need_x ? wq[1] : at::Tensor(), need_w ? xq[0] : at::Tensor(),
@@ -503,7 +508,7 @@ struct MxLinear : public torch::autograd::Function<MxLinear> {
         ctx->saved_data["x_sizes"] = x.sizes().vec();
         ctx->saved_data["n"] = n;
         ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)x.scalar_type(), (int64_t)weight.scalar_type(),
-                                                        b.has_value() ? (int64_t)bias->scalar_type() : 0};
+                                                        b.has_value() && b->defined() ? (int64_t)bias->scalar_type() : 0};
         return mx_shaped(y, x.sizes());
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
@@ -548,7 +553,7 @@ at::Tensor mx_linear_packed(const at::Tensor& x, const at::Tensor& payload, cons
     const int64_t k = x.size(-1), n = payload.size(0);
     at::Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, k});
     const std::vector<at::Tensor> q = mx_quantized(x2, format);
-    at::Tensor y = mx_matmul(q[0], q[1], payload, scales, x2.size(0), n, k, format, format, bias);
+    at::Tensor y = mx_matmul(q[0], q[1], payload, scales, x2.size(0), n, k, format, format, mx_bias(bias));
     return mx_shaped(y, x.sizes());
 }
 

@@ -198,7 +198,8 @@ def _mx_quantize(x: Tensor, elem_format: int):
 
 def mx_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, elem_format: int = 0) -> Tensor:
     """``x @ weight.T + bias`` on microscaled operands: ``x`` ``[..., in]`` and ``weight`` ``[out, in]`` are quantised in
-    groups of 32 along ``in`` (a multiple of 32) and multiplied as codes; the result is bfloat16.  ``elem_format``: 0 E4M3,
+    groups of 32 along ``in`` (a multiple of 32) and multiplied as codes; the result is bfloat16, and so is the bias that is
+    added to the sums (one of another type is rounded first).  ``elem_format``: 0 E4M3,
     1 E5M2 (bfloat16 inputs), 4 E2M1 (bfloat16 or float32).  A group that holds an infinity or a NaN counts as NaN in whole,
     in the product and in the gradients.  The gradients are straight-through: those of a linear layer
     fed the quantised values, computed from the codes, which are all that the forward pass keeps of ``x`` and ``weight``

@@ -48,3 +48,16 @@ def test_results_can_be_written_in_place(shape, name):
     y = packed(x).add_(r)
     assert y.shape == (*shape[:-1], 32) and torch.equal(y, packed(x) + r) and packed(x).is_contiguous()
     assert torch.equal(torch.autograd.grad(y.float().sum(), r)[0], torch.ones_like(r))
+
+
+@pytest.mark.parametrize("name", ["e4m3", "e2m1"])
+def test_a_packed_layer_may_be_cast_with_the_model_around_it(name):
+    """model.float(), model.double() cast its bias, too: the result stays the same bits"""
+    from mor_b200.nn import MXLinear
+    torch.manual_seed(0)
+    packed = MXLinear(64, 40, device="cuda", elem_format=name).pack()
+    x = torch.randn(5, 64, device="cuda").to(torch.bfloat16)
+    want = packed(x)
+    for dtype in (torch.float32, torch.float64, torch.bfloat16):
+        packed.to(dtype)
+        assert packed.bias.dtype == dtype and torch.equal(packed(x), want)
