@@ -288,6 +288,7 @@ std::vector<at::Tensor> fake_quantize_block_scaling_delayed_t(const at::Tensor& 
 std::vector<at::Tensor> quantize_mx(const at::Tensor& input, int64_t rows, int64_t cols, int64_t bc, int64_t elem_format, bool operand) {
     const c10::cuda::CUDAGuard guard(input.device());
     at::Tensor in = checked_input(input, rows, cols, "quantize_mx");
+    if (reinterpret_cast<uintptr_t>(in.data_ptr()) % 16) in = in.clone();   // a slice of a longer tensor
     TORCH_CHECK(in.scalar_type() == at::kBFloat16, "mor::quantize_mx: bfloat16 input only");
     TORCH_CHECK(bc > 0 && cols % bc == 0, "mor::quantize_mx: block_y must divide dim_y");
     TORCH_CHECK(elem_format == MOR_B200_E4M3 || elem_format == MOR_B200_E5M2 || elem_format == MOR_B200_E2M3,
@@ -470,9 +471,7 @@ std::vector<at::Tensor> mx_quantized(const at::Tensor& x, int64_t format) {
     TORCH_CHECK(x.scalar_type() == at::kBFloat16 && c > 0 && c % 32 == 0,
                 "mor::mx_linear: 8-bit operands are quantised from bfloat16, with a width that is a positive multiple of 32");
     if (r == 0) return {mx_empty({0, c}, at::kByte, x), mx_empty({0, c / 32}, at::kByte, x)};
-    at::Tensor packed = x.contiguous();
-    if (reinterpret_cast<uintptr_t>(packed.data_ptr()) % 16) packed = packed.clone();
-    return quantize_mx(packed, r, c, 32, format, /*operand=*/true);
+    return quantize_mx(x, r, c, 32, format, /*operand=*/true);
 }
 
 // A layer's bias as the product adds it: in binary32 before the result's rounding, from bf16, the result's own precision.

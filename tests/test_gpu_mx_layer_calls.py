@@ -61,3 +61,23 @@ def test_a_packed_layer_may_be_cast_with_the_model_around_it(name):
     for dtype in (torch.float32, torch.float64, torch.bfloat16):
         packed.to(dtype)
         assert packed.bias.dtype == dtype and torch.equal(packed(x), want)
+
+
+@pytest.mark.parametrize("name", ["e4m3", "e5m2", "e2m1"])
+def test_weights_that_lie_anywhere(name):
+    """parameters that are slices of one long tensor, as sharded training has them: the layer takes them, and so does pack()"""
+    from mor_b200.nn import MXLinear
+    import mor
+    torch.manual_seed(0)
+    flat = torch.randn(3 + 40 * 64 + 40, device="cuda").to(torch.bfloat16)
+    want, layer = (MXLinear(64, 40, device="cuda", elem_format=name) for _ in range(2))
+    layer.weight, layer.bias = torch.nn.Parameter(flat[3:-40].view(40, 64)), torch.nn.Parameter(flat[-40:])
+    with torch.no_grad():
+        want.weight.copy_(layer.weight), want.bias.copy_(layer.bias)
+    x = torch.randn(6, 64, device="cuda").to(torch.bfloat16)
+    assert layer.weight.data_ptr() % 16 == 6
+    assert torch.equal(layer(x), want(x)) and torch.equal(layer.pack()(x), want(x))
+    if name != "e2m1":
+        for operand in (False, True):
+            for u, v in zip(mor.ops.quantize_mx(layer.weight.detach(), 40, 64, 32, 0, operand), mor.ops.quantize_mx(want.weight.detach(), 40, 64, 32, 0, operand)):
+                assert torch.equal(u, v)
