@@ -295,6 +295,7 @@ std::vector<at::Tensor> quantize_mx(const at::Tensor& input, int64_t rows, int64
                 "mor::quantize_mx: elem_format must be 0 (E4M3), 1 (E5M2) or 3 (E2M3)");
     at::Tensor payload = torch::empty({rows, cols}, in.options().dtype(torch::kUInt8));
     at::Tensor scales = torch::empty({rows, cols / bc}, in.options().dtype(torch::kUInt8));
+    if (rows == 0) return {payload, scales};
     check_status(mor_b200_quantize_mx(in.data_ptr(), payload.data_ptr(), scales.data_ptr(), rows, cols, (int)bc,
                                       (int)elem_format + (operand ? MOR_B200_MX_OPERAND : 0), cur_stream()),
                  "quantize_mx");
@@ -470,7 +471,6 @@ std::vector<at::Tensor> mx_quantized(const at::Tensor& x, int64_t format) {
     if (format == MOR_B200_MX_E2M1) return quantize_mx_fp4(x, r, c, 32);
     TORCH_CHECK(x.scalar_type() == at::kBFloat16 && c > 0 && c % 32 == 0,
                 "mor::mx_linear: 8-bit operands are quantised from bfloat16, with a width that is a positive multiple of 32");
-    if (r == 0) return {mx_empty({0, c}, at::kByte, x), mx_empty({0, c / 32}, at::kByte, x)};
     return quantize_mx(x, r, c, 32, format, /*operand=*/true);
 }
 
@@ -516,8 +516,9 @@ struct MxLinear : public torch::autograd::Function<MxLinear> {
         const int64_t format = ctx->saved_data["format"].toInt(), n = ctx->saved_data["n"].toInt();
         const std::vector<int64_t> sizes = ctx->saved_data["x_sizes"].toIntVector(), types = ctx->saved_data["types"].toIntVector();
         const int64_t k = sizes.back();
-        at::Tensor g = grads[0].dim() == 2 ? grads[0] : grads[0].reshape({-1, n});
-        const int64_t m = g.size(0);
+        int64_t m = 1;   // counted, since a layer of no outputs leaves nothing to infer it from
+        for (size_t i = 0; i + 1 < sizes.size(); ++i) m *= sizes[i];
+        at::Tensor g = grads[0].dim() == 2 ? grads[0] : grads[0].reshape({m, n});
         int64_t pitch = 0;
         g = mx_rows(g, pitch).narrow(1, 0, n);   // packed once where its rows do not fit, for all that read it
         auto typed = [](at::Tensor t, int64_t type) { return t.scalar_type() == (at::ScalarType)type ? t : t.to((at::ScalarType)type); };

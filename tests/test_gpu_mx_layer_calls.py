@@ -81,3 +81,16 @@ def test_weights_that_lie_anywhere(name):
         for operand in (False, True):
             for u, v in zip(mor.ops.quantize_mx(layer.weight.detach(), 40, 64, 32, 0, operand), mor.ops.quantize_mx(want.weight.detach(), 40, 64, 32, 0, operand)):
                 assert torch.equal(u, v)
+
+
+@pytest.mark.parametrize("name", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("shape", [(64,), (5, 64), (2, 3, 64), (0, 64), (2, 0, 64)])
+def test_a_layer_of_no_outputs(shape, name):
+    from mor_b200.nn import MXLinear
+    with pytest.warns(UserWarning, match="zero-element"):
+        layer = MXLinear(64, 0, device="cuda", elem_format=name)
+    x = torch.randn(*shape, device="cuda").to(torch.bfloat16).requires_grad_()
+    y = layer(x)
+    y.backward(torch.empty_like(y))
+    assert y.shape == (*shape[:-1], 0) and x.grad.shape == x.shape and not bool(x.grad.any())
+    assert layer.weight.grad.shape == (0, 64) and layer.bias.grad.shape == (0,) and layer.pack()(x).shape == y.shape
