@@ -283,10 +283,13 @@ inline PairWork pair_work(int64_t tiles, int sms) {
 }
 
 // How many CTAs of a cluster share the sum over k of a tile, when single CTAs take tiles of 128 x (n per tile): as many as leave each
-// an SM of its own and four steps.
+// an SM of its own and four steps.  A cluster lies within one group of the card's SMs, so of those with one CTA an SM 74 of two are
+// resident at a time, but 32 of four (34 are not) and 15 of eight (16 are not), and the ones that wait take a second round:
+// one token x 2048 x 4096 E4M3 (16 tiles) in eighths 9.5 us, in quarters 6.2; x 4352 (34) in quarters 11.8, in halves 8.4;
+// gradients 128 x 2048 x 4096 24.8 and 15.7, 128 x 4352 x 4096 30.9 and 21.4.
 inline int k_splits(int64_t tiles, int64_t steps, int sms) {
     int s = 1;
-    while (s < 8 && tiles * s * 2 <= sms && steps >= s * 4) s *= 2;
+    while (s < 8 && tiles <= (s == 1 ? sms / 2 : (s == 2 ? 32 : 15)) && steps >= s * 4) s *= 2;
     return s;
 }
 // Pairs of CTAs on 256 x 256 or single ones on 128 x 128?  A pair takes a step in about the time of a single CTA with four
