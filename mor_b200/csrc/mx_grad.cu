@@ -447,6 +447,9 @@ bool make_code_map(CUtensorMap* map, const void* base, int64_t rows, int64_t row
               CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// rows of scales that lie on four bytes are fetched by asynchronous copies, others byte by byte
+inline bool fast_scales(const MxGradArgs& x) { return x.n % 128 == 0 && (reinterpret_cast<uintptr_t>(x.scales) & 3) == 0; }
+
 template <int FMT, int CG, int NB>
 int go(const MxGradArgs& x, cudaStream_t st) {
     using S = GrShape<FMT, CG, NB>;
@@ -463,7 +466,7 @@ int go(const MxGradArgs& x, cudaStream_t st) {
     a.m_tiles = (int)mt; a.n_tiles = (int)nt; a.tiles = (int)(mt * nt);
     a.ksteps = (int)((x.k + kTK - 1) / kTK);
     a.across = x.across;
-    a.fast_scales = a.groups % 4 == 0 && (reinterpret_cast<uintptr_t>(x.scales) & 3) == 0;
+    a.fast_scales = fast_scales(x);
     a.splits = 1;
     int grid;
     if constexpr (CG == 2) {
@@ -494,7 +497,7 @@ int go(const MxGradArgs& x, cudaStream_t st) {
 
 template <int FMT>
 int pick(const MxGradArgs& x, cudaStream_t st) {
-    return takes_pairs(x.m, x.n, (x.k + kTK - 1) / kTK, sm_count()) ? go<FMT, 2, 128>(x, st) : go<FMT, 1, 128>(x, st);
+    return takes_pairs(x.m, x.n, (x.k + kTK - 1) / kTK, sm_count(), fast_scales(x) ? 24 : 14) ? go<FMT, 2, 128>(x, st) : go<FMT, 1, 128>(x, st);
 }
 
 }  // namespace

@@ -30,6 +30,7 @@ struct MmArgs {
 };
 
 constexpr int kPRows = 128;
+constexpr int kPairsBelow = 14;   // steps that splitting the sum would save
 
 template <bool FP4, int TN>
 struct MmShape {
@@ -685,7 +686,7 @@ int dispatch(const MxMatmulArgs& x, cudaStream_t st) {
     if (!bind_context()) return kErrLaunch;
     const int64_t row_bytes = FP4 ? x.k / 2 : x.k;
     const bool swap = x.m <= 64;
-    if (!swap && takes_pairs(x.m, x.n, (row_bytes + 127) / 128, sm_count())) return go_pair<FP4>(x, st);
+    if (!swap && takes_pairs(x.m, x.n, (row_bytes + 127) / 128, sm_count(), kPairsBelow)) return go_pair<FP4>(x, st);
     const int tn = !swap ? 128 : (x.m <= 16 ? 16 : (x.m <= 32 ? 32 : 64));
     MmArgs a = {};
     const void *p = swap ? x.b : x.a, *q = swap ? x.a : x.b;
@@ -717,7 +718,7 @@ int dispatch(const MxMatmulArgs& x, cudaStream_t st) {
 
 size_t mx_matmul_workspace(int64_t m, int64_t n, int64_t k, int fp4) {
     const int64_t steps = ((fp4 ? k / 2 : k) + 127) / 128;
-    if (m <= 64 || !takes_pairs(m, n, steps, sm_count()) || !orders_scales(m, n)) return 0;
+    if (m <= 64 || !takes_pairs(m, n, steps, sm_count(), kPairsBelow) || !orders_scales(m, n)) return 0;
     return (size_t)(((m + 127) / 128 + (n + 127) / 128) * scale_blocks(k) * 512);
 }
 

@@ -294,13 +294,18 @@ inline int k_splits(int64_t tiles, int64_t steps, int sms) {
 }
 // Pairs of CTAs on 256 x 256 or single ones on 128 x 128?  A pair takes a step in about the time of a single CTA with four
 // times the result, so pairs win unless few tiles let single CTAs split the sum: each step saved is worth about 0.3 us,
-// meeting in the cluster costs about 4.  Measured on both sides, pairs and single, in us (steps saved): 128 x 4096 x 4096
-// E4M3 14.2 and 12.0 (24), 4-bit 10.6 and 10.9 (12); 256 x 4096 x 4096 E4M3 14.2 and 13.8 (16), 4-bit 10.6 and 11.7 (8);
-// 512 x 1024 x 8192 E4M3 24.3 and 14.6 (48); 100 x 8192 x 8192 4-bit 17.7 and 15.2 (16); 1111 x 1003 x 2080 4-bit 10.3 and
-// 12.6 (5); 1536 x 1536 x 4096 E4M3 15.0 and 19.1 (0); gradients 128 x 4096 x 4096 23.0 and 16.9 (48), 1024^3 9.7 and 12.2 (8).
-inline bool takes_pairs(int64_t m, int64_t n, int64_t steps, int sms) {
+// meeting in the cluster costs about 4 in a product, 7 in a gradient, whose CTAs have more to set up; `limit` is what has to be
+// saved.  Measured on both sides, pairs and single, in us (steps saved).  Products, 14: 128 x 4096 x 4096 E4M3 14.5 and 12.2
+// (24), 4-bit 10.7 and 10.9 (12); 256 x 4096 x 4096 E4M3 14.5 and 13.9 (16), 4-bit 10.7 and 11.7 (8); 128 x 1024 x 2048 E4M3
+// 9.1 and 9.0 (14), 512 x 1024 x 2048 9.1 and 10.5 (12), x 8192 24.3 and 14.8 (48); 100 x 8192 x 8192 4-bit 18.0 and 15.2 (16);
+// 1111 x 1003 x 2080 4-bit 10.5 and 12.6 (5); 1536 x 1536 x 4096 E4M3 15.5 and 20.2 (0).  Gradients, 24: 128 x 4096 x 1024 9.5
+// and 12.4 (12), x 1536 11.8 and 13.2 (18), x 2048 14.1 and 14.0 (24), x 4096 22.7 and 17.2 (48); 256 x 4096 x 2560 16.4 and 17.4
+// (20), x 4096 22.9 and 22.0 (32); 512 x 1024 x 2048 13.5 and 13.8 (24); 128 x 1024 x 1024 8.9 and 10.7 (14).  Gradients whose scale
+// bytes a pair's two warps fetch one by one, 14: 128 x 4000 x 1536 16.0 and 13.6 (18), 256 x 4000 x 1536 16.2 and 15.5 (12),
+// 300 x 992 x 1000 11.4 and 11.8 (12), 1000 x 992 x 1024 11.6 and 13.1 (8).
+inline bool takes_pairs(int64_t m, int64_t n, int64_t steps, int sms, int limit) {
     const int s = k_splits(((m + 127) / 128) * ((n + 127) / 128), steps, sms);
-    return steps - steps / s < 14;
+    return steps - steps / s < limit;
 }
 
 // row-major matrix of bytes (or bf16) with a row pitch, boxes of 128 bytes x box_rows under the 128-byte swizzle; what lies outside reads as zero
