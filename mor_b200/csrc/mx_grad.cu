@@ -5,15 +5,15 @@
 // most) on the way from the staged codes to the operand tile, which costs no global traffic beyond the codes.
 //
 // One kernel, persistent over output tiles.  Per step of 64 k warp 4 requests the gradient's tile by TMA, warp 6 the
-// codes, warps 7-8 their scale bytes, the widening warps turn the codes into the operand tile, warp 5 issues the products, and warps 0-3 write one tile by TMA while the next accumulates (two accumulators).  The
-// gradient's tiles, the codes and the widened tiles pass through rings of their own: codes are let go as soon as they are
+// codes, warps 7-8 their scale bytes, the widening warps turn the codes into the operand tile, warp 5 issues the products, and
+// warps 0-3 write one tile by TMA while the next accumulates (two accumulators).  The gradient's tiles, the codes and the widened tiles pass through rings of their own: codes are let go as soon as they are
 // in registers, and a widened tile is needed only briefly, so most of the shared memory covers the latency of loads.
 // In its large form two CTAs work as a pair on 256 x 256: each loads 128 rows of the gradient and widens 128 columns of W,
 // so every widened element meets 256 rows.
 //
-// A step of a pair is 0.287 us of the tensor core; widening 64 x 128 codes in the same time takes the integer pipe to 46 %
-// and the shared-memory pipe to 62 %.  8192 x 4096 x 4096 E4M3: 188 us in a short run (1.46 PFLOP/s, tensor pipe 73 %
-// active), 213 to 221 us in a long one (power limit).  Two widening groups of four warps take 207 us, three
+// A step of a pair is 0.287 us of the tensor core.  8192 x 4096 x 4096 E4M3: 188 to 195 us in a short run (1.41 to 1.46
+// PFLOP/s), 213 to 227 us in a long one (power limit).  Of its cycles the tensor pipe is active in 76 %, the integer pipe, which
+// widens, in 50 %, the shared-memory pipe in 69 %.  Two widening groups of four warps took 207 us, three
 // 187, four 188 (4096^3 4-bit: 139, 121, 116): what counts is that a group's waits hide behind the others' work.
 #include <algorithm>
 #include <type_traits>

@@ -171,7 +171,8 @@ __global__ void __launch_bounds__(kQThreads) dequantize_kernel(const uint8_t* __
 // out[c] = sum_r g[r, c], the gradient of a bias.  A CTA takes kSumCols columns, lanes of 16 bytes along a row and kSumLanes rows
 // at a time; the CTAs of a cluster share the rows.  Every sum is formed in one order -- a lane's rows, then the lanes, then
 // the CTAs by rank -- so results repeat bit for bit.  Bound by memory and, at these sizes, by starting: 4096 x
-// 4096 9.3 us (3.6 TB/s), 8192 x 4096 14.5 (4.6 TB/s); 256 columns and 512 threads 16.0 and 29.2, 64 and 512 13.4 and 21.8.
+// 4096 9.1 us from memory (3.7 TB/s), 6.5 where the L2 holds the gradient, 8192 x 4096 14.0 (4.8 TB/s) and 9.1; other shapes
+// on an earlier form, 9.3 and 14.5 for this one: 256 columns and 512 threads 16.0 and 29.2, 64 and 512 13.4 and 21.8.
 constexpr int kSumCols = 128, kSumVecs = kSumCols / 8, kSumThreads = 1024, kSumLanes = kSumThreads / kSumVecs;
 __global__ void __launch_bounds__(kSumThreads) column_sums_kernel(const uint16_t* __restrict__ g, int64_t pitch, int64_t rows, int64_t cols,
                                                                     uint16_t* __restrict__ out, int splits) {

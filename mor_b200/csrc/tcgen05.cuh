@@ -254,8 +254,8 @@ __device__ __forceinline__ void tile_place(int t, int m_tiles, int n_tiles, int&
 }
 
 // The work of the pairs of CTAs on 256 x 256 tiles: `rounds` whole tiles each, then the tiles that are left, as halves of 128
-// columns where there are pairs for them: 1024^3 E4M3 (16 tiles) 7.9 us in whole tiles, 6.7 in halves; gradient 512 x 4096 x
-// 4096 27.1 and 23.9; 2560 x 2560 x 8192 4-bit (100 tiles) 28.1 and 26.2.
+// columns where there are pairs for them: 1024^3 E4M3 (16 tiles) 7.9 us in whole tiles, 6.8 in halves; gradient 512 x 4096 x
+// 4096 27.3 and 23.9; 2560 x 2560 x 8192 4-bit (100 tiles) 28.4 and 26.4.
 struct PairWork {
     int pairs, rounds, rest, halves;
     __host__ __device__ int launched() const { return rounds ? pairs : (halves ? 2 * rest : rest); }

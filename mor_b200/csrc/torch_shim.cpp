@@ -490,7 +490,9 @@ at::Tensor mx_shaped(const at::Tensor& y, at::IntArrayRef x_sizes) {
 }
 
 // Straight-through: the gradients are those of a linear layer fed the quantised values, computed from the codes, which are
-// all that the forward pass keeps of the input and the weight.
+// all that the forward pass keeps of the input and the weight.  The operators inside are called as functions, past the
+// dispatcher, which would cost each of seven calls a few microseconds: dispatch modes, tracing and profiles by operator see
+// mx_linear (mx_linear_packed) alone.
 struct MxLinear : public torch::autograd::Function<MxLinear> {
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
                               const std::optional<at::Tensor>& bias, int64_t format) {

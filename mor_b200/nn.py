@@ -204,8 +204,8 @@ def mx_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, elem_for
     in the product and in the gradients.  The gradients are straight-through: those of a linear layer
     fed the quantised values, computed from the codes, which are all that the forward pass keeps of ``x`` and ``weight``
     -- one byte (E2M1: half a byte) and a thirty-second per element in place of two; they have no gradient of their own.
-    Each call quantises the weight it
-    is given; for serving see :meth:`MXLinear.pack`."""
+    Each call quantises the weight it is given; for serving see :meth:`MXLinear.pack`.  To dispatch modes, tracing and
+    profiles by operator the layer is one operator, ``mor::mx_linear``: what it is made of is called inside."""
     if elem_format not in MX_FORMATS.values():
         raise ValueError(f"elem_format must be one of {sorted(MX_FORMATS.values())}, got {elem_format}")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
