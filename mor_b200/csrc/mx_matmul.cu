@@ -6,8 +6,8 @@
 //
 // The tensor core takes such a step of a 256 x 256 tile in 0.287 us (4.3 PFLOP/s 8-bit, 8.6 4-bit over 148 SMs), so a
 // kernel of this kind lives by handing it operands without a pause.  Measured: 8192^3 4-bit 189 to 196 us in a short run (5.6 to
-// 5.8 PFLOP/s, tensor pipe active in 81 % of the cycles), 221 to 229 us in a long one, where the card's power limit lowers the
-// clock; 8192 x 4096 x 4096 E4M3 103 and 121 to 125 us (76 %).  Few tokens are bound by reading the weights: 24 x 16384 x 8192
+// 5.8 PFLOP/s, tensor pipe active in 81 % of the cycles), 219 to 229 us in a long one, where the card's power limit lowers the
+// clock; 8192 x 4096 x 4096 E4M3 103 and 120 to 125 us (76 %).  Few tokens are bound by reading the weights: 24 x 16384 x 8192
 // E4M3 28 us (5.0 TB/s); one token x 4096 x 4096 4-bit by latency, 5.8 us with the weights in L2, 6.2 from memory.
 #include <algorithm>
 
